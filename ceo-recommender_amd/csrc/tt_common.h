@@ -430,10 +430,14 @@ __device__ __forceinline__ AdamCoef adam_coef(double lr, double b1, double b2, d
 }
 
 __device__ __forceinline__ void adam_elem(float& p, float& m, float& v, float g, const AdamCoef& c) {
-  m = m + c.w1 * (g - m);           // lerp, weight < 0.5 branch
-  v = v * c.b2 + (c.c2 * g) * g;    // mul_ + addcmul_
+  // fused multiply-adds spelled out: every kernel that applies Adam (alone, in
+  // the reduction, behind an exchange) gives the same bits, whichever way the
+  // compiler would contract the expressions in each of them
+#pragma clang fp contract(off)
+  m = __builtin_fmaf(c.w1, g - m, m);              // lerp, weight < 0.5 branch
+  v = __builtin_fmaf(c.c2 * g, g, v * c.b2);       // mul_ + addcmul_
   const float denom = sqrtf(v) / c.bc2s + c.eps;
-  p = p + (-c.step_size) * (m / denom);
+  p = __builtin_fmaf(-c.step_size, m / denom, p);
 }
 
 // Adam coefficients of step t, cached in the workspace at slot t & 1 with
