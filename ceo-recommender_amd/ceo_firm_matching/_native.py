@@ -12,7 +12,7 @@ from typing import Optional, Sequence
 
 import torch
 
-TT_ABI_VERSION = 6
+TT_ABI_VERSION = 7
 TT_MAX_CAT = 16
 TT_SLOTS_PER_TOWER = 10
 TT_NUM_OFFSETS = 2 * TT_MAX_CAT + 2 * TT_SLOTS_PER_TOWER + 1
@@ -27,7 +27,11 @@ TT_ERR_WORKSPACE = -4
 TT_FLAG_DETERMINISTIC = 1
 TT_FLAG_DEFER_LATE = 2
 TT_FLAG_LATE_PENDING = 4
-TT_STRUCT_MODEL_DESC, TT_STRUCT_BATCH, TT_STRUCT_ADAM_HP, TT_STRUCT_STATE, TT_STRUCT_AR_PEERS = range(5)
+(TT_STRUCT_MODEL_DESC, TT_STRUCT_BATCH, TT_STRUCT_ADAM_HP, TT_STRUCT_STATE, TT_STRUCT_AR_PEERS,
+ TT_STRUCT_ADAMW_TENSOR, TT_STRUCT_ADAMW_STATE, TT_STRUCT_ADAMW_HP) = range(8)
+TT_BLOCK = 128  # values that share one scale (8-bit states and catalogue rows)
+TT_F32, TT_BF16, TT_F16 = range(3)
+DTYPES = {torch.float32: TT_F32, torch.bfloat16: TT_BF16, torch.float16: TT_F16}
 TT_STATE_BYTES = 32  # tt_state: step_done, step_cur (int64), loss_sum, pad0 (f32), pad1 (int64)
 
 _PKG_PARENT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -40,7 +44,9 @@ EXPORTED = ("tt_abi_version", "tt_struct_size", "tt_stream_copy", "tt_param_coun
             "tt_nce_workspace_bytes", "tt_nce_norms", "tt_nce_forward", "tt_nce_loss", "tt_nce_backward",
             "tt_rank_workspace_bytes", "tt_retrieval_ranks", "tt_step_plan",
             "tt_nce_maxes", "tt_nce_forward_lse", "tt_nce_loss_lse", "tt_nce_backward_lse",
-            "tt_range_push", "tt_range_pop", "tt_randperm")
+            "tt_range_push", "tt_range_pop", "tt_randperm",
+            "tt_adamw_step", "tt_adamw_held", "tt_cat_write", "tt_cat_read", "tt_cat_scores_workspace_bytes",
+            "tt_cat_scores", "tt_cat_dq_workspace_bytes", "tt_cat_dq")
 
 
 class NativeLibraryError(RuntimeError):
@@ -79,6 +85,23 @@ TT_AR_PULL, TT_AR_PUSH = 0, 1  # tt_ar_peers.protocol
 class TTArPeers(ctypes.Structure):  # tt_ar_peers
     _fields_ = [("region", ctypes.c_void_p * TT_AR_MAX_RANKS), ("protocol", ctypes.c_int32),
                 ("reserved", ctypes.c_int32)]
+
+
+class TTAdamWTensor(ctypes.Structure):  # tt_adamw_tensor
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("n", ctypes.c_int64),
+                ("block0", ctypes.c_int64), ("step", ctypes.c_int64), ("dtype", ctypes.c_int64)]
+
+
+class TTAdamWState(ctypes.Structure):  # tt_adamw_state
+    _fields_ = [("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p), ("m_codes", ctypes.c_void_p),
+                ("m_scales", ctypes.c_void_p), ("r_codes", ctypes.c_void_p), ("r_scales", ctypes.c_void_p),
+                ("n_blocks", ctypes.c_int64), ("steps", ctypes.c_void_p), ("coefs", ctypes.c_void_p),
+                ("n_steps", ctypes.c_int64)]
+
+
+class TTAdamWHP(ctypes.Structure):  # tt_adamw_hp
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double)]
 
 
 _LIB: Optional[ctypes.CDLL] = None
@@ -150,6 +173,14 @@ def lib() -> ctypes.CDLL:
         "tt_triplet_workspace_bytes": (I64, [I64, I64, I32]),
         "tt_triplet_forward": (I32, [P, P, I64, I64, I32, I64, F, I64, P, I64, P, P, P, P]),
         "tt_triplet_backward": (I32, [P, P, I64, I64, I32, I64, I64, P, P, P, P, P, P]),
+        "tt_adamw_step": (I32, [P, I32, I32, ctypes.POINTER(TTAdamWState), ctypes.POINTER(TTAdamWHP), U64, P]),
+        "tt_adamw_held": (I32, [ctypes.POINTER(TTAdamWState), P, P, P]),
+        "tt_cat_write": (I32, [P, I32, I64, I64, I32, P, I64, P, P, I64, P, P]),
+        "tt_cat_read": (I32, [P, P, I64, I32, P, I64, I64, P, I32, I64, P]),
+        "tt_cat_scores_workspace_bytes": (I64, [I64, I64, I32]),
+        "tt_cat_scores": (I32, [P, I32, I64, I64, I32, P, P, I64, P, I32, P, I64, P]),
+        "tt_cat_dq_workspace_bytes": (I64, [I64, I64, I32]),
+        "tt_cat_dq": (I32, [P, I32, I64, I64, I64, P, P, I32, P, I32, P, I64, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name, None)
@@ -163,7 +194,8 @@ def lib() -> ctypes.CDLL:
     if v != TT_ABI_VERSION:
         raise NativeLibraryError(f"{LIB_PATH}: ABI version {v}, expected {TT_ABI_VERSION}")
     for which, st in ((TT_STRUCT_MODEL_DESC, TTModelDesc), (TT_STRUCT_BATCH, TTBatch), (TT_STRUCT_ADAM_HP, TTAdamHP),
-                      (TT_STRUCT_AR_PEERS, TTArPeers)):
+                      (TT_STRUCT_AR_PEERS, TTArPeers), (TT_STRUCT_ADAMW_TENSOR, TTAdamWTensor),
+                      (TT_STRUCT_ADAMW_STATE, TTAdamWState), (TT_STRUCT_ADAMW_HP, TTAdamWHP)):
         if L.tt_struct_size(which) != ctypes.sizeof(st):
             raise NativeLibraryError(f"{LIB_PATH}: sizeof({st.__name__}) = {ctypes.sizeof(st)} here, "
                                      f"{L.tt_struct_size(which)} in the library")

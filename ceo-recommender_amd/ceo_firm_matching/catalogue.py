@@ -1,0 +1,231 @@
+"""Embeddings held in 8 bits and scored there (HIP kernels ``tt_cat_*``).
+
+``EmbeddingCatalogue`` keeps the rows that retrieval scores against (the CEO
+embeddings) in e4m3, in blocks of 128 values with a power-of-two scale: a
+quarter of the fp32 rows' bytes, and the product with a block of queries runs
+on the 8-bit matrix cores.  Rows are quantised as they are written and read
+back as the values they stand for.
+
+    cat = EmbeddingCatalogue(n_ceos, 256, device="cuda")
+    cat.write(ceo_embeddings)                    # rows 0, 1, ...
+    cat.write(changed, rows=where)               # rows[i] takes changed[i]
+    s = cat.scores(firm_embeddings)              # [m, n_ceos]
+    s.backward(ds)                               # gradient of firm_embeddings
+
+Values: every rounding to e4m3 is to nearest even, off by at most 2^-4 of the
+value (2^-10 of the block's scale near zero).  Infinities and NaN are held as
+NaN and reach only the scores of their own row.  The queries are rounded the
+same way inside ``scores``; the gradient passes that rounding through unchanged
+and is ``ds @ read()`` with sums in 32 bits.  The catalogue itself gets no
+gradient.
+
+On CPU tensors the same values come from torch ops.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+from . import block8
+
+
+def _check_dtype(dtype: torch.dtype, what: str):
+    if dtype not in N.DTYPES:
+        raise NotImplementedError(f"{what}: float32, bfloat16 or float16, got {dtype}")
+
+
+def _rows_2d(x: torch.Tensor, d: int, what: str) -> torch.Tensor:
+    """[m, d] with unit stride in a row and rows that do not overlap."""
+    if x.dim() != 2 or x.shape[1] != d:
+        raise ValueError(f"{what}: expected [rows, {d}], got {tuple(x.shape)}")
+    if (d > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < d):
+        x = x.contiguous()
+    return x
+
+
+class _ScoresFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, codes, scales, d, n, out_dtype):
+        ctx.save_for_backward(codes, scales)
+        ctx.meta = (d, n, q.dtype)
+        m = q.shape[0]
+        if q.device.type != "cuda":
+            qv = block8.decode(*block8.encode(q), d)
+            return (qv @ block8.decode(codes[:n], scales[:n], d).t()).to(out_dtype)
+        out = torch.empty(m, n, dtype=out_dtype, device=q.device)
+        L = N.lib()
+        wsb = int(L.tt_cat_scores_workspace_bytes(m, n, d))
+        if wsb < 0:
+            N.check(wsb, "tt_cat_scores_workspace_bytes")
+        with torch.cuda.device(q.device):
+            ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
+            N.check(L.tt_cat_scores(q.data_ptr(), N.DTYPES[q.dtype], m, q.stride(0), d, codes.data_ptr(),
+                                    scales.data_ptr(), n, out.data_ptr(), N.DTYPES[out_dtype], ws.data_ptr(), wsb,
+                                    N.stream_ptr(q.device)), "tt_cat_scores")
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, ds):
+        codes, scales = ctx.saved_tensors
+        d, n, dtype = ctx.meta
+        m = ds.shape[0]
+        if ds.device.type != "cuda":
+            dq = ds.to(torch.float32) @ block8.decode(codes[:n], scales[:n], d)
+            return dq.to(dtype), None, None, None, None, None
+        if (n > 1 and ds.stride(1) != 1) or (m > 1 and ds.stride(0) < n):
+            ds = ds.contiguous()
+        dq = torch.empty(m, d, dtype=dtype, device=ds.device)
+        L = N.lib()
+        wsb = int(L.tt_cat_dq_workspace_bytes(m, n, d))
+        if wsb < 0:
+            N.check(wsb, "tt_cat_dq_workspace_bytes")
+        with torch.cuda.device(ds.device):
+            ws = torch.empty(wsb, dtype=torch.uint8, device=ds.device)
+            N.check(L.tt_cat_dq(ds.data_ptr(), N.DTYPES[ds.dtype], m, ds.stride(0), n, codes.data_ptr(),
+                                scales.data_ptr(), d, dq.data_ptr(), N.DTYPES[dtype], ws.data_ptr(), wsb,
+                                N.stream_ptr(ds.device)), "tt_cat_dq")
+        return dq, None, None, None, None, None
+
+
+class EmbeddingCatalogue:
+    """``capacity`` rows of ``dim`` values in e4m3 blocks of 128.
+
+    ``codes`` uint8 [capacity, kp] (kp = dim rounded up to 128, padding zero)
+    and ``scales`` uint8 [capacity, kp / 128] (2^(byte - 127)) are the storage:
+    ``torch.save`` them, and rebuild with :meth:`from_storage`.  Rows never
+    written are zero.  Calls run on the current stream of the catalogue's
+    device; writes from several streams have to be ordered by the caller.
+    """
+
+    def __init__(self, capacity: int, dim: int, device=None):
+        capacity, dim = int(capacity), int(dim)
+        if capacity < 0 or not 1 <= dim <= 1 << 20:
+            raise ValueError(f"EmbeddingCatalogue: capacity >= 0 and 1 <= dim <= {1 << 20}, got {capacity}, {dim}")
+        dev = torch.device("cpu" if device is None else device)
+        nkb = block8.blocks_of(dim)
+        self._bind(torch.zeros(capacity, nkb * block8.BLOCK, dtype=torch.uint8, device=dev),
+                   torch.full((capacity, nkb), 127, dtype=torch.uint8, device=dev), dim)
+
+    @classmethod
+    def from_storage(cls, codes: torch.Tensor, scales: torch.Tensor, dim: int) -> "EmbeddingCatalogue":
+        """A catalogue on existing storage (shared, not copied)."""
+        dim = int(dim)
+        if not 1 <= dim <= 1 << 20:
+            raise ValueError(f"EmbeddingCatalogue: 1 <= dim <= {1 << 20}, got {dim}")
+        nkb = block8.blocks_of(dim)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.device != scales.device:
+            raise ValueError("from_storage: codes and scales are uint8 tensors on one device")
+        if codes.dim() != 2 or tuple(scales.shape) != (codes.shape[0], nkb) or codes.shape[1] != nkb * block8.BLOCK:
+            raise ValueError(f"from_storage: codes [rows, {nkb * block8.BLOCK}] and scales [rows, {nkb}] for dim {dim}, "
+                             f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
+            raise ValueError("from_storage: contiguous storage, codes on a 16-byte boundary")
+        self = cls.__new__(cls)
+        self._bind(codes, scales, dim)
+        return self
+
+    def _bind(self, codes, scales, dim):
+        self.codes, self.scales, self.dim = codes, scales, dim
+        self.capacity, self.device = codes.shape[0], codes.device
+        # which mention of a row an indexed write keeps; zero between calls
+        self._owner = (torch.zeros(self.capacity, dtype=torch.int32, device=codes.device)
+                       if codes.device.type == "cuda" else None)
+
+    # -- rows of a call -------------------------------------------------------
+    def _check_rows(self, rows, m: int, what: str):
+        if rows is None:
+            return None
+        if rows.dim() != 1 or rows.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"{what}: rows is a 1-d int64 or int32 tensor")
+        if rows.device != self.device:
+            raise ValueError(f"{what}: rows on {rows.device}, the catalogue on {self.device}")
+        if m >= 0 and rows.shape[0] != m:
+            raise ValueError(f"{what}: {rows.shape[0]} row numbers for {m} rows")
+        return rows.to(torch.int64).contiguous()
+
+    def _check_range(self, start: int, m: int, what: str):
+        if start < 0 or m < 0 or start + m > self.capacity:
+            raise ValueError(f"{what}: rows {start} .. {start + m} of {self.capacity}")
+
+    def write(self, emb: torch.Tensor, rows: Optional[torch.Tensor] = None, start: int = 0) -> None:
+        """Quantise ``emb`` [m, dim] into rows ``start ..`` or, with ``rows``
+        [m], into those.  Row numbers outside the catalogue are left out (a
+        padded batch uses -1); a row named twice takes its last mention."""
+        emb = _rows_2d(emb.detach(), self.dim, "write")
+        _check_dtype(emb.dtype, "write")
+        if emb.device != self.device:
+            raise ValueError(f"write: embeddings on {emb.device}, the catalogue on {self.device}")
+        m, start = emb.shape[0], int(start)
+        rows = self._check_rows(rows, m, "write")
+        if rows is None:
+            self._check_range(start, m, "write")
+        elif start:
+            raise ValueError("write: rows or start, not both")
+        if m == 0:
+            return
+        torch.autograd.graph.increment_version((self.codes, self.scales))  # a backward that saved the old rows must notice
+        if self.device.type != "cuda":
+            codes, scales = block8.encode(emb)
+            if rows is None:
+                self.codes[start:start + m], self.scales[start:start + m] = codes, scales
+                return
+            last = {int(r): i for i, r in enumerate(rows.tolist()) if 0 <= r < self.capacity}
+            if last:
+                r, i = torch.tensor(list(last.keys())), torch.tensor(list(last.values()))
+                self.codes[r], self.scales[r] = codes[i], scales[i]
+            return
+        with torch.cuda.device(self.device):
+            N.check(N.lib().tt_cat_write(emb.data_ptr(), N.DTYPES[emb.dtype], m, emb.stride(0), self.dim, N.ptr(rows),
+                                         start, self.codes.data_ptr(), self.scales.data_ptr(), self.capacity,
+                                         N.ptr(self._owner), N.stream_ptr(self.device)), "tt_cat_write")
+
+    def read(self, rows: Optional[torch.Tensor] = None, start: int = 0, count: Optional[int] = None,
+             dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values rows ``start .. start + count`` (default: to the end) or
+        ``rows`` stand for, [m, dim]; row numbers outside the catalogue read
+        as zeros.  float32 and bfloat16 hold every value exactly."""
+        _check_dtype(dtype, "read")
+        rows = self._check_rows(rows, -1, "read")
+        start = int(start)
+        if rows is not None:
+            if start or count is not None:
+                raise ValueError("read: rows or a range, not both")
+            m = rows.shape[0]
+        else:
+            m = self.capacity - start if count is None else int(count)
+            self._check_range(start, m, "read")
+        if self.device.type != "cuda":
+            if rows is None:
+                return block8.decode(self.codes[start:start + m], self.scales[start:start + m], self.dim).to(dtype)
+            ok = (rows >= 0) & (rows < self.capacity)
+            out = torch.zeros(m, self.dim)
+            out[ok] = block8.decode(self.codes[rows[ok]], self.scales[rows[ok]], self.dim)
+            return out.to(dtype)
+        with torch.cuda.device(self.device):
+            out = torch.empty(m, self.dim, dtype=dtype, device=self.device)
+            N.check(N.lib().tt_cat_read(self.codes.data_ptr(), self.scales.data_ptr(), self.capacity, self.dim,
+                                        N.ptr(rows), start, m, out.data_ptr(), N.DTYPES[dtype], self.dim,
+                                        N.stream_ptr(self.device)), "tt_cat_read")
+        return out
+
+    def scores(self, queries: torch.Tensor, count: Optional[int] = None,
+               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """Inner products of ``queries`` [..., dim] with the first ``count``
+        rows (default: all), [..., count], in ``dtype`` (default: the
+        queries').  Differentiable in the queries."""
+        dtype = queries.dtype if dtype is None else dtype
+        _check_dtype(queries.dtype, "scores")
+        _check_dtype(dtype, "scores")
+        if queries.device != self.device:
+            raise ValueError(f"scores: queries on {queries.device}, the catalogue on {self.device}")
+        if queries.dim() < 1 or queries.shape[-1] != self.dim:
+            raise ValueError(f"scores: expected [..., {self.dim}], got {tuple(queries.shape)}")
+        n = self.capacity if count is None else int(count)
+        self._check_range(0, n, "scores")
+        q = _rows_2d(queries.reshape(-1, self.dim), self.dim, "scores")
+        s = _ScoresFn.apply(q, self.codes, self.scales, self.dim, n, dtype)
+        return s.reshape(*queries.shape[:-1], n)

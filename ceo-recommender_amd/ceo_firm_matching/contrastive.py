@@ -11,7 +11,8 @@ SURVEY 8a rows a18/a19, BASELINE cfg 5:
   the ranks of a process group (one GPU each): all-gather of the CEO rows,
   all-reduce of the column sums and of the loss, reduce-scatter of dC.
 * ``retrieval_ranks`` / ``compute_retrieval_metrics`` (contrastive.py:275-332):
-  rank of the true match among all candidates, recall@1/5/k, MRR, median rank.
+  rank of the true match among all candidates, recall@1/5/k, MRR, median rank
+  (``storage="e4m3"``, ``catalogue_ranks``: against embeddings held in 8 bits).
 * ``semi_hard_negative_mining`` (contrastive.py:141-192): triplet loss with
   semi-hard negatives as one fused similarity GEMM + masked-min kernel
   (tt_triplet_*) instead of a per-row Python loop.
@@ -37,8 +38,11 @@ import torch.optim as optim
 from torch.utils.data import DataLoader
 
 from . import _native as N
+from .catalogue import EmbeddingCatalogue
 from .config import Config
 from .model import _POISON_WS, CEOFirmMatcher
+from .optim import AdamW
+
 
 def _status_bad(status: torch.Tensor) -> bool:
     """Underflowed softmax sums in the shared-shift pass (host read)."""
@@ -382,11 +386,35 @@ def retrieval_ranks_rows(f: torch.Tensor, c: torch.Tensor, row0: int = 0) -> tor
     return ranks
 
 
-def retrieval_ranks(firm_emb: torch.Tensor, ceo_emb: torch.Tensor, cap: Optional[int] = 5000) -> torch.Tensor:
+def catalogue_ranks(firm_emb: torch.Tensor, catalogue: EmbeddingCatalogue, row0: int = 0) -> torch.Tensor:
+    """``retrieval_ranks_rows`` against embeddings held in 8 bits: 1-based rank
+    of catalogue row row0 + i among all rows for firm row i, by the scores in
+    32 bits (a block of firms at a time, so that the scores stay small)."""
+    m, n = firm_emb.shape[0], catalogue.capacity
+    if row0 < 0 or row0 + m > n:
+        raise ValueError("catalogue_ranks: firm rows must map onto catalogue rows row0..row0+m")
+    ranks = torch.empty(m, dtype=torch.int32, device=firm_emb.device)
+    step = max(1, min(m, (1 << 28) // max(n, 1)))
+    for i in range(0, m, step):
+        s = catalogue.scores(firm_emb[i:i + step].detach(), dtype=torch.float32)
+        own = torch.arange(row0 + i, row0 + i + s.shape[0], device=s.device)
+        ranks[i:i + step] = (s > s.gather(1, own[:, None])).sum(dim=1).to(torch.int32) + 1
+    return ranks
+
+
+def retrieval_ranks(firm_emb: torch.Tensor, ceo_emb: torch.Tensor, cap: Optional[int] = 5000,
+                    storage: Optional[str] = None) -> torch.Tensor:
     """Ranks over the first N = min(rows, cap) pairs, as the reference
-    (contrastive.py:306-322); ``cap=None`` ranks all pairs."""
+    (contrastive.py:306-322); ``cap=None`` ranks all pairs.
+    ``storage="e4m3"`` ranks as a catalogue in 8 bits would answer."""
+    if storage not in (None, "e4m3"):
+        raise ValueError(f"retrieval_ranks: storage is None or 'e4m3', got {storage!r}")
     N_ = firm_emb.size(0) if cap is None else min(firm_emb.size(0), cap)
-    return retrieval_ranks_rows(firm_emb[:N_], ceo_emb[:N_], 0)
+    if storage is None:
+        return retrieval_ranks_rows(firm_emb[:N_], ceo_emb[:N_], 0)
+    catalogue = EmbeddingCatalogue(N_, ceo_emb.shape[1], device=ceo_emb.device)
+    catalogue.write(ceo_emb[:N_])
+    return catalogue_ranks(firm_emb[:N_], catalogue)
 
 
 def metrics_from_ranks(ranks: torch.Tensor, top_k: int = 10) -> Dict[str, float]:
@@ -401,14 +429,15 @@ def metrics_from_ranks(ranks: torch.Tensor, top_k: int = 10) -> Dict[str, float]
 
 
 def compute_retrieval_metrics(model, data_dict: Dict, config: Config, top_k: int = 10,
-                              cap: Optional[int] = 5000) -> Dict[str, float]:
-    """Reference contrastive.py:275-332 (``cap=None``: no 5000-row cap)."""
+                              cap: Optional[int] = 5000, storage: Optional[str] = None) -> Dict[str, float]:
+    """Reference contrastive.py:275-332 (``cap=None``: no 5000-row cap;
+    ``storage="e4m3"``: the CEO embeddings held in 8 bits)."""
     model.eval()
     with torch.no_grad():
         dev = config.DEVICE
         fe, ce = model.get_embeddings(data_dict['firm_numeric'].to(dev), data_dict['firm_cat'].to(dev),
                                       data_dict['ceo_numeric'].to(dev), data_dict['ceo_cat'].to(dev))
-        ranks = retrieval_ranks(fe, ce, cap=cap)
+        ranks = retrieval_ranks(fe, ce, cap=cap, storage=storage)
     return metrics_from_ranks(ranks, top_k)
 
 
@@ -441,7 +470,8 @@ class ContrastiveCEOFirmMatcher(nn.Module):
 # --------------------------------------------------------------------------
 def train_contrastive(train_loader: DataLoader, val_loader: DataLoader, metadata: Dict[str, int], config: Config,
                       contrastive_weight: float = 0.3, temperature: float = 0.07,
-                      use_triplet: bool = False) -> ContrastiveCEOFirmMatcher:
+                      use_triplet: bool = False, optimizer: str = "adam",
+                      weight_decay: float = 1e-2) -> ContrastiveCEOFirmMatcher:
     """Train the two-tower model on (1 - a) * weighted MSE + a * InfoNCE (or
     semi-hard triplet) loss -- reference contrastive.py:197-272, same
     signature, same prints, same batch order (the loader is iterated as is).
@@ -449,10 +479,18 @@ def train_contrastive(train_loader: DataLoader, val_loader: DataLoader, metadata
     On a HIP device the towers run forward and backward in the fused kernels
     (one autograd node for both encoders), InfoNCE / triplet mining in the
     similarity kernels; the projector heads, the match score and Adam are
-    ATen ops.  Loss totals stay on the device until an epoch is printed
+    ATen ops.  ``optimizer="adamw"`` / ``"adamw8bit"`` takes the multi-tensor
+    AdamW (``optim.AdamW``, decay ``weight_decay``) with states in 32 / 8 bits
+    in Adam's place.  Loss totals stay on the device until an epoch is printed
     (the reference syncs three times per step with ``.item()``)."""
+    if optimizer not in ("adam", "adamw", "adamw8bit"):
+        raise ValueError(f"train_contrastive: optimizer is 'adam', 'adamw' or 'adamw8bit', got {optimizer!r}")
     model = ContrastiveCEOFirmMatcher(metadata, config).to(config.DEVICE)
-    optimizer = optim.Adam(model.parameters(), lr=config.LEARNING_RATE)
+    if optimizer == "adam":
+        opt = optim.Adam(model.parameters(), lr=config.LEARNING_RATE)
+    else:
+        opt = AdamW(model.parameters(), lr=config.LEARNING_RATE, weight_decay=weight_decay,
+                    state_bits=8 if optimizer == "adamw8bit" else 32)
 
     print(f"Training Contrastive Two-Tower on {config.DEVICE}")
     print(f"  Contrastive weight: {contrastive_weight}")
@@ -466,7 +504,7 @@ def train_contrastive(train_loader: DataLoader, val_loader: DataLoader, metadata
         n_batches = 0
         for batch in train_loader:
             batch = {k: v.to(dev) for k, v in batch.items()}
-            optimizer.zero_grad()
+            opt.zero_grad()
             match_score, firm_proj, ceo_proj = model(batch['firm_numeric'], batch['firm_cat'],
                                                      batch['ceo_numeric'], batch['ceo_cat'])
             mse_loss = (batch['weights'] * (match_score - batch['target']) ** 2).mean()
@@ -476,7 +514,7 @@ def train_contrastive(train_loader: DataLoader, val_loader: DataLoader, metadata
                 cl_loss = info_nce_loss(firm_proj, ceo_proj, temperature)
             loss = (1 - contrastive_weight) * mse_loss + contrastive_weight * cl_loss
             loss.backward()
-            optimizer.step()
+            opt.step()
             totals += torch.stack([loss.detach(), mse_loss.detach(), cl_loss.detach().to(mse_loss.dtype)]).double()
             n_batches += 1
         if epoch % 5 == 0:

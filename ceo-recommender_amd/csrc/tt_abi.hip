@@ -875,6 +875,9 @@ int64_t tt_struct_size(int32_t which) {
     case TT_STRUCT_ADAM_HP: return (int64_t)sizeof(tt_adam_hp);
     case TT_STRUCT_STATE: return (int64_t)sizeof(tt_state);
     case TT_STRUCT_AR_PEERS: return (int64_t)sizeof(tt_ar_peers);
+    case TT_STRUCT_ADAMW_TENSOR: return (int64_t)sizeof(tt_adamw_tensor);
+    case TT_STRUCT_ADAMW_STATE: return (int64_t)sizeof(tt_adamw_state);
+    case TT_STRUCT_ADAMW_HP: return (int64_t)sizeof(tt_adamw_hp);
     default: return -1;
   }
 }

@@ -1,0 +1,228 @@
+// Host side of the operators beside the two-tower path (a translation unit of
+// its own): argument checks and launches of the multi-tensor AdamW step and
+// of the 8-bit embedding catalogue, behind the C-ABI of include/ceo_tt.h.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "tt_adamw.hip"
+#include "tt_catalogue.hip"
+
+namespace tt {
+
+static int ops_launch_check() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? TT_OK : (int)e;
+}
+static bool dtype_ok(int64_t dt) { return dt == TT_F32 || dt == TT_BF16 || dt == TT_F16; }
+static unsigned grid_for(int64_t work, int64_t per_block, int64_t most) {
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>((work + per_block - 1) / per_block, most));
+}
+
+// F(std::integral_constant) for an element type known at run time
+template <typename F>
+static void with_dtype(int32_t dt, F f) {
+  if (dt == TT_F32)
+    f(std::integral_constant<int, TT_F32>{});
+  else if (dt == TT_BF16)
+    f(std::integral_constant<int, TT_BF16>{});
+  else
+    f(std::integral_constant<int, TT_F16>{});
+}
+
+}  // namespace tt
+
+using namespace tt;
+
+extern "C" {
+
+int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t state_bits,
+                      const tt_adamw_state* state, const tt_adamw_hp* hp, uint64_t seed, tt_stream_t stream) {
+  if (!state || !hp || n_tensors < 0 || (n_tensors > 0 && !tensors)) return TT_ERR_ARG;
+  if (state_bits != 8 && state_bits != 32) return TT_ERR_UNSUPPORTED;
+  if (!(hp->beta1 >= 0.0 && hp->beta1 < 1.0 && hp->beta2 >= 0.0 && hp->beta2 < 1.0 && hp->eps >= 0.0)) return TT_ERR_ARG;
+  if (!std::isfinite(hp->lr) || !std::isfinite(hp->weight_decay)) return TT_ERR_ARG;
+  if (state->n_blocks < 0 || state->n_blocks > (int64_t)UINT32_MAX) return TT_ERR_ARG;  // the hash takes 32 bits
+  if (state->steps && !state->coefs) return TT_ERR_ARG;
+  int64_t values = 0;
+  for (int32_t i = 0; i < n_tensors; ++i) {
+    const tt_adamw_tensor& t = tensors[i];
+    if (t.n < 0 || !dtype_ok(t.dtype)) return TT_ERR_ARG;
+    if (t.n == 0) continue;
+    const int64_t align = t.dtype == TT_F32 ? 4 : 2;
+    if (!t.param || !t.grad || (uintptr_t)t.param % align || (uintptr_t)t.grad % align) return TT_ERR_ARG;
+    const int64_t nb = (t.n - 1) / TT_BLOCK + 1;
+    if (t.block0 < 0 || nb > state->n_blocks || t.block0 > state->n_blocks - nb) return TT_ERR_ARG;
+    if (state->steps ? t.step < 0 || t.step >= state->n_steps : t.step < 1) return TT_ERR_ARG;
+    values += t.n;
+  }
+  if (values == 0) return TT_OK;
+  if (state_bits == 32 ? !state->exp_avg || !state->exp_avg_sq
+                       : !state->m_codes || !state->m_scales || !state->r_codes || !state->r_scales)
+    return TT_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  AdamwArgs a;
+  a.w1 = (float)(1.0 - hp->beta1);
+  a.b2 = (float)hp->beta2;
+  a.c2 = (float)(1.0 - hp->beta2);
+  a.eps = (float)hp->eps;
+  a.decay = (float)(1.0 - hp->lr * hp->weight_decay);
+  a.m = state->exp_avg;
+  a.v = state->exp_avg_sq;
+  a.mc = state->m_codes;
+  a.ms = state->m_scales;
+  a.rc = state->r_codes;
+  a.rs = state->r_scales;
+  a.steps = state->steps;
+  a.coefs = (AdamwCoef*)state->coefs;
+  a.lr = hp->lr;
+  a.b1d = hp->beta1;
+  a.b2d = hp->beta2;
+  a.seed = seed;
+  int64_t chunk = ADAMW_STRIDE;
+  int64_t last_step = 0;
+  AdamwCoef last{};
+  for (int32_t from = 0; from < n_tensors;) {
+    int64_t chunks = 0;
+    a.n_t = 0;
+    for (; from < n_tensors && a.n_t < ADAMW_LIST; ++from) {
+      const tt_adamw_tensor& t = tensors[from];
+      if (t.n == 0) continue;
+      const int64_t c = (t.n + chunk - 1) / chunk;
+      if (c > INT32_MAX / 2) return TT_ERR_UNSUPPORTED;
+      if (chunks + c > INT32_MAX / 2) break;
+      const int k = a.n_t++;
+      a.p[k] = t.param;
+      a.g[k] = t.grad;
+      a.n[k] = t.n;
+      a.blk[k] = t.block0;
+      a.dtype[k] = (uint8_t)t.dtype;
+      a.first[k] = (int32_t)chunks;
+      if (state->steps) {
+        a.c[k] = AdamwCoef{0.f, 0.f, (uint32_t)t.step, 0u};
+      } else {
+        if (t.step != last_step) last = adamw_coef(hp->lr, hp->beta1, hp->beta2, seed, last_step = t.step);
+        a.c[k] = last;
+      }
+      chunks += c;
+    }
+    if (a.n_t == 0) break;
+    for (int k = a.n_t; k < ADAMW_LIST; ++k) a.first[k] = INT32_MAX;
+    a.chunk = (int32_t)chunk;
+    if (state->steps) hipLaunchKernelGGL(k_adamw_advance, dim3(1), dim3(ADAMW_LIST), 0, s, a);
+    if (state_bits == 32)
+      hipLaunchKernelGGL(k_adamw<32>, dim3((unsigned)chunks), dim3(ADAMW_THREADS), 0, s, a);
+    else
+      hipLaunchKernelGGL(k_adamw<8>, dim3((unsigned)chunks), dim3(ADAMW_THREADS), 0, s, a);
+    if (const int rc = ops_launch_check()) return rc;
+  }
+  return TT_OK;
+}
+
+int32_t tt_adamw_held(const tt_adamw_state* state, void* m, void* r, tt_stream_t stream) {
+  if (!state || state->n_blocks < 0) return TT_ERR_ARG;
+  if (state->n_blocks == 0) return TT_OK;
+  if (!state->m_codes || !state->m_scales || !state->r_codes || !state->r_scales || !m || !r) return TT_ERR_ARG;
+  const int64_t n8 = state->n_blocks * b8::LANES;
+  hipLaunchKernelGGL(k_adamw_held, dim3(grid_for(n8, 256, 8192), 2), dim3(256), 0, (hipStream_t)stream, state->m_codes,
+                     state->m_scales, state->r_codes, state->r_scales, m, r, n8);
+  return ops_launch_check();
+}
+
+// shared checks of the catalogue calls: sizes whose products stay in 63 bits
+static bool cat_sizes_ok(int64_t rows, int32_t d) { return rows >= 0 && rows <= ((int64_t)1 << 40) && d >= 1 && d <= (1 << 20); }
+static int cat_blocks(int32_t d) { return (d + TT_BLOCK - 1) / TT_BLOCK; }
+
+int32_t tt_cat_write(const void* x, int32_t dtype, int64_t m, int64_t ldx, int32_t d, const int64_t* rows, int64_t row0,
+                     uint8_t* codes, uint8_t* scales, int64_t capacity, int32_t* owner, tt_stream_t stream) {
+  if (!cat_sizes_ok(m, d) || !cat_sizes_ok(capacity, d) || !dtype_ok(dtype) || (m > 1 && ldx < d)) return TT_ERR_ARG;
+  if (rows && (m >= INT32_MAX || (m > 0 && !owner))) return TT_ERR_ARG;  // a row's owner is a place in 31 bits
+  if (!rows && (row0 < 0 || row0 > capacity - m)) return TT_ERR_ARG;
+  if (m == 0 || capacity == 0) return TT_OK;
+  if (!x || !codes || !scales) return TT_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  const CatRows r{rows, row0, capacity};
+  const int nkb = cat_blocks(d);
+  if (rows) hipLaunchKernelGGL(k_cat_own, dim3(grid_for(m, 256, 4096)), dim3(256), 0, s, r, m, owner);
+  with_dtype(dtype, [&](auto t) {
+    hipLaunchKernelGGL(k_cat_write<decltype(t)::value>, dim3(grid_for(m * nkb, 16, 16384)), dim3(256), 0, s, x, m, ldx,
+                       d, nkb, r, codes, scales, rows ? owner : nullptr);
+  });
+  if (rows) hipLaunchKernelGGL(k_cat_disown, dim3(grid_for(m, 256, 4096)), dim3(256), 0, s, r, m, owner);
+  return ops_launch_check();
+}
+
+int32_t tt_cat_read(const uint8_t* codes, const uint8_t* scales, int64_t capacity, int32_t d, const int64_t* rows,
+                    int64_t row0, int64_t m, void* out, int32_t dtype, int64_t ldo, tt_stream_t stream) {
+  if (!cat_sizes_ok(m, d) || !cat_sizes_ok(capacity, d) || !dtype_ok(dtype) || (m > 1 && ldo < d)) return TT_ERR_ARG;
+  if (!rows && (row0 < 0 || row0 > capacity - m)) return TT_ERR_ARG;
+  if (m == 0) return TT_OK;
+  if (!out || (capacity > 0 && (!codes || !scales))) return TT_ERR_ARG;
+  const CatRows r{rows, row0, capacity};
+  const int nkb = cat_blocks(d);
+  with_dtype(dtype, [&](auto t) {
+    hipLaunchKernelGGL(k_cat_read<decltype(t)::value>, dim3(grid_for(m * nkb, 16, 16384)), dim3(256), 0,
+                       (hipStream_t)stream, codes, scales, r, m, d, nkb, out, ldo);
+  });
+  return ops_launch_check();
+}
+
+int64_t tt_cat_scores_workspace_bytes(int64_t m, int64_t n, int32_t d) {
+  if (!cat_sizes_ok(m, d) || !cat_sizes_ok(n, d)) return TT_ERR_ARG;
+  const int64_t nkb = cat_blocks(d);
+  return m * nkb * TT_BLOCK + (m * nkb + 255) / 256 * 256;  // codes | scales
+}
+
+int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int32_t d, const uint8_t* codes,
+                      const uint8_t* scales, int64_t n, void* out, int32_t out_dtype, void* ws, int64_t ws_bytes,
+                      tt_stream_t stream) {
+  if (!cat_sizes_ok(m, d) || !cat_sizes_ok(n, d) || !dtype_ok(dtype) || !dtype_ok(out_dtype) || (m > 1 && ldq < d))
+    return TT_ERR_ARG;
+  if (m == 0 || n == 0) return TT_OK;
+  if (!q || !codes || !scales || !out || !ws) return TT_ERR_ARG;
+  if (ws_bytes < tt_cat_scores_workspace_bytes(m, n, d)) return TT_ERR_WORKSPACE;
+  const int nkb = cat_blocks(d);
+  const int64_t nt = (n + 63) / 64, mt = (m + 63) / 64;
+  if (mt > INT32_MAX / nt) return TT_ERR_UNSUPPORTED;
+  hipStream_t s = (hipStream_t)stream;
+  uint8_t* qc = (uint8_t*)ws;
+  uint8_t* qs = qc + m * nkb * TT_BLOCK;
+  const CatRows r{nullptr, 0, m};
+  with_dtype(dtype, [&](auto t) {
+    hipLaunchKernelGGL(k_cat_write<decltype(t)::value>, dim3(grid_for(m * nkb, 16, 16384)), dim3(256), 0, s, q, m, ldq,
+                       d, nkb, r, qc, qs, (int32_t*)nullptr);
+  });
+  with_dtype(out_dtype, [&](auto t) {
+    hipLaunchKernelGGL(k_cat_scores<decltype(t)::value>, dim3((unsigned)(mt * nt)), dim3(256), 0, s, qc, qs, m, codes,
+                       scales, n, nkb, out, nt);
+  });
+  return ops_launch_check();
+}
+
+int64_t tt_cat_dq_workspace_bytes(int64_t m, int64_t n, int32_t d) {
+  if (!cat_sizes_ok(m, d) || !cat_sizes_ok(n, d)) return TT_ERR_ARG;
+  return 0;
+}
+
+int32_t tt_cat_dq(const void* ds, int32_t ds_dtype, int64_t m, int64_t lds, int64_t n, const uint8_t* codes,
+                  const uint8_t* scales, int32_t d, void* dq, int32_t dq_dtype, void* ws, int64_t ws_bytes,
+                  tt_stream_t stream) {
+  if (!cat_sizes_ok(m, d) || !cat_sizes_ok(n, d) || !dtype_ok(ds_dtype) || !dtype_ok(dq_dtype) || (m > 1 && lds < n))
+    return TT_ERR_ARG;
+  if (m == 0) return TT_OK;
+  if (!dq || (n > 0 && (!ds || !codes || !scales))) return TT_ERR_ARG;
+  const int64_t need = tt_cat_dq_workspace_bytes(m, n, d);
+  if (need > 0 && (!ws || ws_bytes < need)) return TT_ERR_WORKSPACE;
+  const int nkb = cat_blocks(d), ct = (d + 15) / 16;
+  const int64_t mt = (m + 15) / 16;
+  if (mt > INT32_MAX / ct) return TT_ERR_UNSUPPORTED;
+  with_dtype(ds_dtype, [&](auto t) {
+    with_dtype(dq_dtype, [&](auto u) {
+      hipLaunchKernelGGL((k_cat_dq<decltype(t)::value, decltype(u)::value>), dim3((unsigned)(mt * ct)), dim3(64), 0,
+                         (hipStream_t)stream, ds, m, lds, n, codes, scales, d, nkb, dq, ct);
+    });
+  });
+  return ops_launch_check();
+}
+
+}  // extern "C"

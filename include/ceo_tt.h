@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define TT_ABI_VERSION 6
+#define TT_ABI_VERSION 7
 #define TT_MAX_CAT 16      /* categorical columns per tower */
 
 /* status codes */
@@ -153,6 +153,9 @@ void tt_range_pop(void);
 #define TT_STRUCT_ADAM_HP 2
 #define TT_STRUCT_STATE 3
 #define TT_STRUCT_AR_PEERS 4
+#define TT_STRUCT_ADAMW_TENSOR 5
+#define TT_STRUCT_ADAMW_STATE 6
+#define TT_STRUCT_ADAMW_HP 7
 int64_t tt_struct_size(int32_t which);
 
 /* Flat parameter arena size (floats) and per-parameter offsets. */
@@ -468,6 +471,86 @@ int32_t tt_train_step_dp(const tt_model_desc* d, float* params, float* buffers, 
                          void* ws, int64_t ws_bytes, float* grad, float* exp_avg, float* exp_avg_sq,
                          const tt_ar_peers* peers, int32_t rank, int32_t world, int32_t co_ranks,
                          int32_t* err, int64_t wait_us, tt_stream_t stream);
+
+/* ---- AdamW over many tensors (ABI 7) --------------------------------------
+ * One decoupled-weight-decay Adam step over a list of tensors of any sizes in
+ * one launch per 64 tensors, beside tt_adam_apply's one flat arena:
+ *   m' = m + (1 - b1)(g - m);  v' = b2 v + (1 - b2) g^2;
+ *   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+ * in 32 bits whatever the tensors' type, p' rounded once.  The states live in
+ * arenas of blocks of TT_BLOCK values: tensor i's values start at block
+ * block0 and its last block is padded (the padding stays zero).
+ *   state_bits 32: exp_avg, exp_avg_sq (fp32 [n_blocks * TT_BLOCK]).
+ *   state_bits 8:  m as sign + e4m3 (m_codes), sqrt(v) as unsigned e4m4
+ *     (r_codes), each block with a power-of-two scale 2^(byte - 127) chosen
+ *     from its largest finite magnitude; both are rounded up or down with the
+ *     probability of what is cut off, by a hash of (seed, t, value's place),
+ *     so a step is repeatable; a positive root is never held as zero;
+ *     infinities and NaN are held as NaN.
+ * t = tensors[i].step, or with `steps` (device int64, capturable): that
+ * entry's counter steps[tensors[i].step], which this call increments.       */
+#define TT_BLOCK 128
+#define TT_F32 0
+#define TT_BF16 1
+#define TT_F16 2
+typedef struct tt_adamw_tensor {
+  void* param;
+  const void* grad;      /* of the parameter's type, contiguous */
+  int64_t n;             /* values */
+  int64_t block0;        /* its first block of the state arenas */
+  int64_t step;          /* t >= 1, or the index of its counter in `steps` */
+  int64_t dtype;         /* TT_F32, TT_BF16, TT_F16 */
+} tt_adamw_tensor;
+typedef struct tt_adamw_state {
+  float *exp_avg, *exp_avg_sq;              /* state_bits 32 */
+  uint8_t *m_codes, *m_scales;              /* state_bits 8 */
+  uint8_t *r_codes, *r_scales;
+  int64_t n_blocks;
+  int64_t* steps;                           /* nullable */
+  float* coefs;                             /* [4 * n_steps] floats, with `steps` */
+  int64_t n_steps;
+} tt_adamw_state;
+typedef struct tt_adamw_hp {
+  double lr, beta1, beta2, eps, weight_decay;
+} tt_adamw_hp;
+int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t state_bits,
+                      const tt_adamw_state* state, const tt_adamw_hp* hp, uint64_t seed,
+                      tt_stream_t stream);
+/* The values that 8-bit states stand for, exactly, in bfloat16:
+ * m, r [n_blocks * TT_BLOCK] (r = sqrt(exp_avg_sq)).                        */
+int32_t tt_adamw_held(const tt_adamw_state* state, void* m, void* r, tt_stream_t stream);
+
+/* ---- embedding catalogue in 8 bits (ABI 7) ---------------------------------
+ * Rows of d values in e4m3, each block of TT_BLOCK values with a power-of-two
+ * scale 2^(byte - 127), the smallest that holds the block's largest finite
+ * magnitude (not below 2^-100).  codes [capacity, kp], scales [capacity,
+ * kp / TT_BLOCK], kp = d rounded up to TT_BLOCK (padding codes are zero).
+ * Infinities and NaN are held as NaN.  Row i of a call is catalogue row
+ * rows[i] (device int64), or row0 + i when rows == NULL; rows outside
+ * [0, capacity) are left out of a write and read as zeros.  A row named twice
+ * in one write takes the values of its last mention; owner [capacity] (device
+ * int32, zero before the first call and after each) is needed with rows.    */
+int32_t tt_cat_write(const void* x, int32_t dtype, int64_t m, int64_t ldx, int32_t d,
+                     const int64_t* rows, int64_t row0, uint8_t* codes, uint8_t* scales,
+                     int64_t capacity, int32_t* owner, tt_stream_t stream);
+int32_t tt_cat_read(const uint8_t* codes, const uint8_t* scales, int64_t capacity, int32_t d,
+                    const int64_t* rows, int64_t row0, int64_t m, void* out, int32_t dtype,
+                    int64_t ldo, tt_stream_t stream);
+/* scores [m, n] = Q^ C^^T: queries q [m, d] in blocks as above, against the
+ * catalogue's first n rows; sums in 32 bits, rounded once to out_dtype.
+ * ws: tt_cat_scores_workspace_bytes(m, n, d) (the queries' codes).          */
+int64_t tt_cat_scores_workspace_bytes(int64_t m, int64_t n, int32_t d);
+int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int32_t d,
+                      const uint8_t* codes, const uint8_t* scales, int64_t n, void* out,
+                      int32_t out_dtype, void* ws, int64_t ws_bytes, tt_stream_t stream);
+/* dq [m, d] = dS C^ (the queries' rounding passes the gradient through; the
+ * catalogue gets none).  ds [m, n] of ds_dtype with row stride lds; sums in
+ * 32 bits, in an order that only the sizes decide.
+ * ws: tt_cat_dq_workspace_bytes(m, n, d).                                   */
+int64_t tt_cat_dq_workspace_bytes(int64_t m, int64_t n, int32_t d);
+int32_t tt_cat_dq(const void* ds, int32_t ds_dtype, int64_t m, int64_t lds, int64_t n,
+                  const uint8_t* codes, const uint8_t* scales, int32_t d, void* dq,
+                  int32_t dq_dtype, void* ws, int64_t ws_bytes, tt_stream_t stream);
 
 #ifdef __cplusplus
 }
