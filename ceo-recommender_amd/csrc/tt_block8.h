@@ -119,6 +119,21 @@ __device__ __forceinline__ void st8n(void* p, int64_t i, int k, const float (&x)
 }
 
 // ---- e4m3, rounded to nearest even (the catalogue) -------------------------
+// 8 values under a scale byte -> 8 code bytes; infinities become NaN: e4m3 has none
+__device__ __forceinline__ u32x2 encode8_scaled(const float (&x)[8], uint32_t byte) {
+  const float inv = inv_scale(byte);
+  float y[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t a = __float_as_uint(x[k]) & 0x7FFFFFFFu;
+    y[k] = finite_bits(a) ? x[k] * inv : __uint_as_float(0x7FC00000u);
+  }
+  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
+  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], hi, true);
+  return (u32x2){(uint32_t)lo, (uint32_t)hi};
+}
 // 8 values of a block spread over 16 lanes -> 8 code bytes; every lane of the
 // row gets the block's scale byte
 __device__ __forceinline__ u32x2 encode8(const float (&x)[8], uint32_t& byte) {
@@ -129,18 +144,7 @@ __device__ __forceinline__ u32x2 encode8(const float (&x)[8], uint32_t& byte) {
     amax = max(amax, finite_bits(a) ? a : 0u);
   }
   byte = (uint32_t)scale_byte(row_max16(amax), CARRY_M);
-  const float inv = inv_scale(byte);
-  float y[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {  // infinities become NaN: e4m3 has none
-    const uint32_t a = __float_as_uint(x[k]) & 0x7FFFFFFFu;
-    y[k] = finite_bits(a) ? x[k] * inv : __uint_as_float(0x7FC00000u);
-  }
-  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
-  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], hi, true);
-  return (u32x2){(uint32_t)lo, (uint32_t)hi};
+  return encode8_scaled(x, byte);
 }
 __device__ __forceinline__ void decode4(uint32_t w, float s, float* x) {
   const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);

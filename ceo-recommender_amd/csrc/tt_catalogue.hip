@@ -74,7 +74,8 @@ __global__ __launch_bounds__(256) void k_cat_read(const uint8_t* codes, const ui
 
 // ---------------------------------------------------------------------------
 // scores = Q^ C^^T.  Lane l supplies 32 bytes of operand row l & 15 for a block
-// of 128 (which 32 is the same for both operands, so any order of k is right);
+// of 128: 16-byte chunks l >> 4 and (l >> 4) + 4 of the row (the same for both
+// operands, so this order of k is right; a load then takes 64 bytes of a row);
 // C: lane l holds C[row = 4 (l >> 4) + reg][column = l & 15].
 //
 // Results in 16 bits: v_mfma_scale_f32_16x16x128_f8f6f4, one instruction a
@@ -94,11 +95,11 @@ __device__ __forceinline__ f32x4 mfma_block8(const i32x8& a, const i32x8& b, con
 }
 // 8 codes and their block's scale -> bf16, exact
 __device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t lo, uint32_t hi, float s) {
-  float x[8];
-  b8::decode8((u32x2){lo, hi}, s, x);
   u32x4 w;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) w[k] = pk_bf16(x[2 * k], x[2 * k + 1]);
+  w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));
+  w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true));
+  w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false));
+  w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
   return __builtin_bit_cast(bf16x8, w);
 }
 __device__ __forceinline__ f32x4 mfma_block_bf16(const i32x8& a, const i32x8& b, f32x4 c, int sa, int sb) {
@@ -110,51 +111,375 @@ __device__ __forceinline__ f32x4 mfma_block_bf16(const i32x8& a, const i32x8& b,
   return c;
 }
 
+__device__ __forceinline__ i32x8 frag_of(const u32x4& lo, const u32x4& hi) {
+  return (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+// from the 128 bytes of a row at p (16-byte aligned)
+__device__ __forceinline__ i32x8 row_frag(const uint8_t* p, int g) {
+  return frag_of(*reinterpret_cast<const u32x4*>(p + 16 * g), *reinterpret_cast<const u32x4*>(p + 16 * g + 64));
+}
+
+// LDS image of 128-byte rows (one block of codes each): 16-byte chunk c of row
+// r lies at chunk c ^ (r & 7), so that 8 lanes that read one chunk of 8
+// consecutive rows touch all 32 banks once.
+constexpr int ROWB = TT_BLOCK;
+__device__ __forceinline__ int lds_chunk(int row, int c) { return row * ROWB + ((c ^ (row & 7)) << 4); }
+__device__ __forceinline__ i32x8 lds_frag(const uint8_t* s, int row, int g) {
+  return frag_of(*reinterpret_cast<const u32x4*>(s + lds_chunk(row, g)),
+                 *reinterpret_cast<const u32x4*>(s + lds_chunk(row, g + 4)));
+}
+// 16 bytes a lane from global memory straight into LDS at base + 16 lane
+__device__ __forceinline__ void ld_lds16(const uint8_t* g, uint8_t* s) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                   (__attribute__((address_space(3))) void*)s, 16, 0, 0);
+}
+__device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// a barrier that orders LDS alone: loads and stores of global memory stay in flight
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 template <int DT>
-__global__ __launch_bounds__(256) void k_cat_scores(const uint8_t* q, const uint8_t* qs, int64_t m,
-                                                    const uint8_t* codes, const uint8_t* scales, int64_t n, int nkb,
-                                                    void* out, int64_t n_tiles) {
+__device__ __forceinline__ f32x4 mfma_block(const i32x8& a, const i32x8& b, const f32x4& c, int sa, int sb) {
+  return DT == TT_F32 ? mfma_block_bf16(a, b, c, sa, sb) : mfma_block8(a, b, c, sa, sb);
+}
+
+// A wave's tile of 16 QT queries x 16 IT catalogue rows, stored row by row:
+// lane (r, g) holds 4 consecutive columns of row r; it is turned in the wave's
+// own LDS so that 16-byte pieces of whole rows go out (pieces at any address:
+// rows of odd length start anywhere).
+template <int DT, int IT, int QT> constexpr int tile_lds() { return 16 * QT * (16 * IT * b8::Elem<DT>::SIZE + 16); }
+// WHOLE: all 16 IT columns exist and 64 rows of the result span less than 2 GiB
+template <int DT, int IT, int QT, bool WHOLE>
+__device__ __forceinline__ void store_tile(uint8_t* so, const f32x4 (&acc)[IT][QT], void* out, int64_t m0, int64_t m,
+                                           int64_t n0, int64_t n) {
   using namespace b8;
-  const int l = lane_id(), w = wave_id();
-  const int64_t tm = (int64_t)blockIdx.x / n_tiles, tn = (int64_t)blockIdx.x % n_tiles;
-  const int64_t m0 = tm * 64 + (w >> 1) * 32, n0 = tn * 64 + (w & 1) * 32;
-  f32x4 acc[2][2];
+  constexpr int ES = Elem<DT>::SIZE, LDO = 16 * IT * ES + 16;
+  constexpr int PER = 16 / ES, LPR = 16 * IT / PER;  // values of a piece, pieces of a row
+  const int l = lane_id(), r = l & 15, g = l >> 4;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < QT; ++j)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = zero4();
-  int64_t rc[2], rq[2];
+    for (int i = 0; i < IT; ++i) {
+      uint8_t* at = so + (16 * j + r) * LDO + (16 * i + 4 * g) * ES;
+      const f32x4 v = acc[i][j];
+      if constexpr (DT == TT_F32)
+        *reinterpret_cast<f32x4*>(at) = v;
+      else if constexpr (DT == TT_BF16)
+        *reinterpret_cast<u32x2*>(at) = (u32x2){pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
+      else
+        *reinterpret_cast<u32x2*>(at) = (u32x2){float_to_half_bits(v[0]) | (uint32_t)float_to_half_bits(v[1]) << 16,
+                                                float_to_half_bits(v[2]) | (uint32_t)float_to_half_bits(v[3]) << 16};
+    }
+  __builtin_amdgcn_wave_barrier();
+  const int rows = (int)min((int64_t)(16 * QT), m - m0), cols = (int)min((int64_t)(16 * IT), n - n0);
+  uint8_t* const base = (uint8_t*)out + (m0 * n + n0) * ES;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    rc[i] = min(n0 + 16 * i + (l & 15), n - 1);
-    rq[i] = min(m0 + 16 * i + (l & 15), m - 1);
+  for (int k = 0; k < (16 * QT * LPR + 63) / 64; ++k) {
+    const int u = k * 64 + l, row = u / LPR, c = (u % LPR) * PER;
+    const uint8_t* from = so + row * LDO + c * ES;
+    if constexpr (WHOLE) {
+      // no branch: the loop over tiles then knows how many stores follow the
+      // next tile's loads and waits for the loads alone
+      const uint32_t off = row < rows && u < 16 * QT * LPR ? (uint32_t)row * (uint32_t)(n * ES) + (uint32_t)(c * ES) : 0x80000000u;
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(base, (short)0, 0x7FFFFFFF, 0x00020000);
+      __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4*>(from), rs, (int)off, 0, 0);
+    } else if (row < rows && c < cols) {
+      uint8_t* to = base + ((int64_t)row * n + c) * ES;
+      if (c + PER <= cols) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(from);
+        __builtin_memcpy(to, &v, 16);
+      } else {
+        for (int e = 0; e < cols - c; ++e) __builtin_memcpy(to + e * ES, from + e * ES, ES);
+      }
+    }
   }
-  for (int kb = 0; kb < nkb; ++kb) {
-    i32x8 a[2], b[2];
-    int sa[2], sb[2];
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Few blocks a row (or few queries): a wave keeps 16 QT queries in registers
+// and walks over the catalogue, 16 IT rows at a time, straight from global
+// memory: no barrier, and the next rows' loads fly while this tile is stored.
+// The 4 waves of a workgroup take neighbouring row groups, so that a query's
+// results go out in pieces of 64 IT values.
+struct StreamArgs {
+  const void* q;            // raw queries (ENC) or their codes
+  const uint8_t* qs;        // their scale bytes (not ENC)
+  const uint8_t *codes, *scales;
+  void* out;
+  int64_t m, n, ldq;
+  int d, nkb, q_dtype;
+  int64_t panels, strips, per;  // workgroup t of an XCD's share: panel t / strips, strip t % strips
+};
+
+// codes and scale byte of this lane's query in the block from k: values 16 g .. and 64 + 16 g ..
+template <int QDT>
+__device__ __forceinline__ i32x8 encode_query(const void* q, int64_t at, int k, int d, bool live, int& byte) {
+  using namespace b8;
+  float x[4][8];
+  uint32_t amax = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      __builtin_memcpy(&a[i], codes + (rc[i] * nkb + kb) * BLK + (l >> 4) * 32, 32);
-      __builtin_memcpy(&b[i], q + (rq[i] * nkb + kb) * BLK + (l >> 4) * 32, 32);
-      sa[i] = scales[rc[i] * nkb + kb];
-      sb[i] = qs[rq[i] * nkb + kb];
+  for (int c = 0; c < 4; ++c) {
+    const int kc = k + 8 * (c & 1) + 64 * (c >> 1);
+    ld8n<QDT>(q, at + kc, live ? max(0, min(8, d - kc)) : 0, x[c]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t a = __float_as_uint(x[c][e]) & 0x7FFFFFFFu;
+      amax = max(amax, finite_bits(a) ? a : 0u);
+    }
+  }
+  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
+  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
+  byte = scale_byte(amax, CARRY_M);
+  i32x8 w;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const u32x2 p = encode8_scaled(x[c], (uint32_t)byte);
+    w[2 * c] = (int)p[0];
+    w[2 * c + 1] = (int)p[1];
+  }
+  return w;
+}
+
+// NKB: blocks a row, 0: any number, with the queries' codes read again for every tile
+template <int DT, int IT, int QT, int NKB, bool ENC>
+__global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs a) {
+  using namespace b8;
+  constexpr int KB = NKB ? NKB : 1;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * tile_lds<DT, IT, QT>()];
+  const int l = lane_id(), w = wave_id(), r = l & 15, g = l >> 4;
+  uint8_t* const so = lds + w * tile_lds<DT, IT, QT>();
+  const int64_t t = (int64_t)(blockIdx.x & 7) * a.per + (blockIdx.x >> 3);
+  if (t >= a.panels * a.strips) return;
+  const int64_t panel = t / a.strips, strip = t % a.strips;
+  const int64_t m0 = panel * 16 * QT, n = a.n;
+  const int nkb = NKB ? NKB : a.nkb;
+  // this strip's groups of 64 IT rows
+  const int64_t groups = (n + 64 * IT - 1) / (64 * IT);
+  const int64_t g0 = groups * strip / a.strips, g1 = groups * (strip + 1) / a.strips;
+
+  const uint8_t* qrow[QT];
+  const uint8_t* qsrow[QT];
+  i32x8 b[KB][QT];
+  int sb[KB][QT];
+#pragma unroll
+  for (int j = 0; j < QT; ++j) {
+    const int64_t row = m0 + 16 * j + r, at = min(row, a.m - 1);
+    if constexpr (!ENC) {
+      qrow[j] = (const uint8_t*)a.q + at * nkb * ROWB;
+      qsrow[j] = a.qs + at * nkb;
+    }
+    if constexpr (NKB > 0) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        if constexpr (ENC) {
+          const int k = kb * BLK + 16 * g;
+          if (a.q_dtype == TT_F32)
+            b[kb][j] = encode_query<TT_F32>(a.q, at * a.ldq, k, a.d, row < a.m, sb[kb][j]);
+          else if (a.q_dtype == TT_BF16)
+            b[kb][j] = encode_query<TT_BF16>(a.q, at * a.ldq, k, a.d, row < a.m, sb[kb][j]);
+          else
+            b[kb][j] = encode_query<TT_F16>(a.q, at * a.ldq, k, a.d, row < a.m, sb[kb][j]);
+        } else {
+          b[kb][j] = row_frag(qrow[j] + kb * ROWB, g);
+          sb[kb][j] = qsrow[j][kb];
+        }
+      }
+    }
+  }
+
+  if constexpr (NKB > 0) {
+    i32x8 x[KB][IT];
+    int sa[KB][IT];
+    auto load = [&](int64_t n0) {
+      const int last = (int)min((int64_t)(16 * IT), n - n0) - 1;
+      const uint8_t* c0 = a.codes + n0 * (KB * ROWB);
+      const uint8_t* s0 = a.scales + n0 * KB;
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const uint32_t row = (uint32_t)min(16 * i + r, last);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          x[kb][i] = row_frag(c0 + (row * KB + kb) * ROWB, g);
+          sa[kb][i] = s0[row * KB + kb];
+        }
+      }
+    };
+    f32x4 acc[IT][QT];
+    auto multiply = [&]() {
+#pragma unroll
+      for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int j = 0; j < QT; ++j) acc[i][j] = zero4();
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+          for (int j = 0; j < QT; ++j)
+            acc[i][j] = mfma_block<DT>(x[kb][i], b[kb][j], acc[i][j], sa[kb][i], sb[kb][j]);
+    };
+    int64_t n0 = (g0 * 4 + w) * 16 * IT;
+    const int64_t end = min(n, g1 * 64 * IT);
+    // whole tiles first; addresses of the one after the last stay inside the catalogue
+    const int64_t whole = n * Elem<DT>::SIZE * 64 < 0x7FFFFFFF ? end - 16 * IT : -1;
+    if (n0 < end) load(n0);
+    while (n0 <= whole) {
+      multiply();
+      const int64_t at = n0;
+      n0 += 64 * IT;
+      load(min(n0, n - 1));  // in flight while this tile is stored
+      store_tile<DT, IT, QT, true>(so, acc, a.out, m0, a.m, at, n);
+    }
+    while (n0 < end) {
+      multiply();
+      store_tile<DT, IT, QT, false>(so, acc, a.out, m0, a.m, n0, n);
+      n0 += 64 * IT;
+      if (n0 < end) load(n0);
+    }
+  } else {
+    for (int64_t u = g0; u < g1; ++u) {
+      const int64_t n0 = (u * 4 + w) * 16 * IT;
+      if (n0 >= n) break;
+      const int last = (int)min((int64_t)(16 * IT), n - n0) - 1;
+      const uint8_t* c0 = a.codes + n0 * nkb * ROWB;
+      const uint8_t* s0 = a.scales + n0 * nkb;
+      f32x4 acc[IT][QT];
+#pragma unroll
+      for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int j = 0; j < QT; ++j) acc[i][j] = zero4();
+      for (int kb = 0; kb < nkb; ++kb) {
+        i32x8 x[IT], y[QT];
+        int sx[IT], sy[QT];
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+          const int64_t row = min(16 * i + r, last);
+          x[i] = row_frag(c0 + (row * nkb + kb) * ROWB, g);
+          sx[i] = s0[row * nkb + kb];
+        }
+#pragma unroll
+        for (int j = 0; j < QT; ++j) {
+          y[j] = row_frag(qrow[j] + (int64_t)kb * ROWB, g);
+          sy[j] = qsrow[j][kb];
+        }
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+          for (int j = 0; j < QT; ++j) acc[i][j] = mfma_block<DT>(x[i], y[j], acc[i][j], sx[i], sy[j]);
+      }
+      store_tile<DT, IT, QT, false>(so, acc, a.out, m0, a.m, n0, n);
+    }
+  }
+}
+
+// a wave's 64 x 64 results, STORE_J 16-query tiles at a time
+template <int DT> constexpr int STORE_J = DT == TT_F32 ? 2 : 4;
+template <int DT, bool WHOLE>
+__device__ __forceinline__ void store_wave(uint8_t* so, const f32x4 (&acc)[4][4], void* out, int64_t m0, int64_t m,
+                                           int64_t n0, int64_t n) {
+  constexpr int J = STORE_J<DT>;
+#pragma unroll
+  for (int j0 = 0; j0 < 4; j0 += J) {
+    f32x4 y[4][J];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < J; ++j) y[i][j] = acc[i][j0 + j];
+    store_tile<DT, 4, J, WHOLE>(so, y, out, m0 + 16 * j0, m, n0, n);
+  }
+}
+
+// Many queries: one workgroup a tile of 128 queries x 128 catalogue rows, a
+// wave 64 x 64 of it, a block of 128 values staged in LDS at a time.  Nothing is
+// fetched ahead: four workgroups a CU (128 registers a lane, 36 KB) cover each
+// other's loads and stores.  Two of 8 waves that keep 256 queries in registers
+// and stage ahead, with a quarter of the L2 reads, took 460 us where this takes
+// 420 (8192 x 100000 x 256 in bf16): their waves meet at barriers.
+constexpr int CT_M = 128, CT_N = 128;
+
+// Tile of workgroup `id` of 8 * per: XCD x runs workgroups x, x + 8, ... and
+// takes the x-th eighth of the tiles, in panels of `width` column tiles walked
+// over all row tiles: its L2 holds a panel's catalogue rows (512 KB at most)
+// and meets every query once a panel.  Wide panels also write long pieces of
+// the same rows at a time: 8 -> 32 column tiles 338 -> 273 us at 16384 x 32771 x 128.
+__device__ __forceinline__ bool cat_tile(int64_t id, int64_t per, int64_t mt, int64_t nt, int width, int64_t& tm,
+                                         int64_t& tn) {
+  const int64_t t = (id & 7) * per + (id >> 3);
+  if (t >= mt * nt) return false;
+  const int64_t panel = (int64_t)width * mt, p = t / panel, in = t - p * panel;
+  const int64_t cols = min((int64_t)width, nt - p * width);  // the last panel may be narrower
+  tn = p * width + in % cols;
+  tm = in / cols;
+  return true;
+}
+
+template <int DT>
+__global__ __launch_bounds__(256, DT == TT_F32 ? 3 : 4) void k_cat_scores(
+    const uint8_t* __restrict__ q, const uint8_t* __restrict__ qs, int64_t m, const uint8_t* __restrict__ codes,
+    const uint8_t* __restrict__ scales, int64_t n, int nkb, void* out, int64_t mt, int64_t nt, int64_t per, int width) {
+  using namespace b8;
+  constexpr int SO = 4 * tile_lds<DT, 4, STORE_J<DT>>();
+  __shared__ __attribute__((aligned(128))) uint8_t lds[SO > 2 * 128 * ROWB + 256 ? SO : 2 * 128 * ROWB + 256];
+  uint8_t* const sc = lds;               // catalogue rows
+  uint8_t* const sq = lds + CT_N * ROWB; // queries
+  const int l = lane_id(), w = wave_id(), r = l & 15, g = l >> 4;
+  int64_t tm, tn;
+  if (!cat_tile(blockIdx.x, per, mt, nt, width, tm, tn)) return;
+  const int64_t m0 = tm * CT_M, n0 = tn * CT_N;
+  const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
+  const int rows_q = (int)min((int64_t)CT_M, m - m0), rows_c = (int)min((int64_t)CT_N, n - n0);
+
+  // staging: 8 rows a wave and instruction, wave w takes rows 32 w .. 32 w + 31
+  // of both operands; loads past the last row bring zeros
+  const int64_t kp = (int64_t)nkb * ROWB;
+  const uint32_t off = (uint32_t)((l >> 3) * kp + (((l & 7) ^ (l >> 3)) << 4));
+  auto stage = [&](const uint8_t* from, int rows, uint8_t* to) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int first = 32 * w + 8 * i;
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from + first * kp), (short)0,
+                                                        (int)(max(0, rows - first) * kp), 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(to + first * ROWB), 16,
+                                               (int)off, 0, 0, 0);
+    }
+  };
+  const uint8_t *gc = codes + n0 * kp, *gq = q + m0 * kp;
+  // thread t brings the scale byte of catalogue row t or of query t - 128
+  const int srow = (int)threadIdx.x % 128;
+  const uint8_t* gs = (int)threadIdx.x < 128 ? scales + (n0 + min(srow, rows_c - 1)) * nkb : qs + (m0 + min(srow, rows_q - 1)) * nkb;
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = zero4();
+
+  for (int kb = 0; kb < nkb; ++kb) {
+    stage(gc + kb * ROWB, rows_c, sc);
+    stage(gq + kb * ROWB, rows_q, sq);
+    lds[2 * 128 * ROWB + threadIdx.x] = gs[kb];
+    wait_lds_loads();
+    __syncthreads();
+    i32x8 a[4];
+    int sa[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = lds_frag(sc, wn + 16 * i + r, g);
+      sa[i] = lds[2 * 128 * ROWB + wn + 16 * i + r];
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 4; ++j) {
+      const i32x8 b = lds_frag(sq, wm + 16 * j + r, g);
+      const int sb = lds[2 * 128 * ROWB + 128 + wm + 16 * j + r];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        acc[i][j] = DT == TT_F32 ? mfma_block_bf16(a[i], b[j], acc[i][j], sa[i], sb[j])
-                                 : mfma_block8(a[i], b[j], acc[i][j], sa[i], sb[j]);
+      for (int i = 0; i < 4; ++i) acc[i][j] = mfma_block<DT>(a[i], b, acc[i][j], sa[i], sb);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t row = m0 + 16 * j + (l & 15), col = n0 + 16 * i + 4 * (l >> 4) + e;
-        if (row < m && col < n) st1<DT>(out, row * n + col, acc[i][j][e]);
-      }
+
+  store_wave<DT, false>(lds + w * tile_lds<DT, 4, STORE_J<DT>>(), acc, out, m0 + wm, m, n0 + wn, n);
 }
 
 // ---------------------------------------------------------------------------

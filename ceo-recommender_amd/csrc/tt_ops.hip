@@ -4,6 +4,8 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <mutex>
+#include <type_traits>
 
 #include "tt_adamw.hip"
 #include "tt_catalogue.hip"
@@ -167,11 +169,57 @@ int32_t tt_cat_read(const uint8_t* codes, const uint8_t* scales, int64_t capacit
   return ops_launch_check();
 }
 
+// queries that a streaming wave encodes itself: no workspace, one launch
+static bool cat_encodes(int64_t m, int nkb) { return m <= 16 && nkb <= 4; }
+
 int64_t tt_cat_scores_workspace_bytes(int64_t m, int64_t n, int32_t d) {
   if (!cat_sizes_ok(m, d) || !cat_sizes_ok(n, d)) return TT_ERR_ARG;
   const int64_t nkb = cat_blocks(d);
+  if (cat_encodes(m, (int)nkb)) return 0;
   return m * nkb * TT_BLOCK + (m * nkb + 255) / 256 * 256;  // codes | scales
 }
+
+}  // extern "C"
+
+namespace tt {
+template <int DT, int IT, int QT, int NKB, bool ENC>
+static int launch_stream(StreamArgs& a, hipStream_t s) {
+  a.panels = (a.m + 16 * QT - 1) / (16 * QT);
+  const int64_t groups = (a.n + 64 * IT - 1) / (64 * IT);
+  const int64_t want = 512 * (QT == 4 ? 1 : 4 / IT);
+  a.strips = std::max<int64_t>(1, std::min(groups, (want + a.panels - 1) / a.panels));
+  if (a.panels > INT32_MAX / 16 / a.strips) return TT_ERR_UNSUPPORTED;
+  a.per = (a.panels * a.strips + 7) / 8;
+  hipLaunchKernelGGL((k_cat_stream<DT, IT, QT, NKB, ENC>), dim3((unsigned)(8 * a.per)), dim3(256), 0, s, a);
+  return TT_OK;
+}
+template <int DT, int IT, int QT, bool ENC>
+static int stream_by_blocks(StreamArgs& a, hipStream_t s) {
+  switch (a.nkb) {
+    case 1: return launch_stream<DT, IT, QT, 1, ENC>(a, s);
+    case 2: return launch_stream<DT, IT, QT, 2, ENC>(a, s);
+    case 3: if constexpr (QT < 4) return launch_stream<DT, IT, QT, 3, ENC>(a, s);
+    case 4: if constexpr (QT < 4) return launch_stream<DT, IT, QT, 4, ENC>(a, s);
+  }
+  if constexpr (!ENC) return launch_stream<DT, IT, QT, 0, false>(a, s);
+  return TT_ERR_UNSUPPORTED;
+}
+template <int DT>
+static int launch_scores(StreamArgs& a, hipStream_t s) {
+  if (cat_encodes(a.m, a.nkb)) return stream_by_blocks<DT, 1, 1, true>(a, s);
+  if (a.m <= 16) return stream_by_blocks<DT, 1, 1, false>(a, s);
+  if (a.m <= 32) return stream_by_blocks<DT, 2, 2, false>(a, s);
+  if (a.m <= 64) return stream_by_blocks<DT, 4, 4, false>(a, s);
+  const int64_t nt = (a.n + CT_N - 1) / CT_N, mt = (a.m + CT_M - 1) / CT_M;
+  if (mt > INT32_MAX / 8 / nt) return TT_ERR_UNSUPPORTED;
+  const int64_t per = (mt * nt + 7) / 8;
+  hipLaunchKernelGGL(k_cat_scores<DT>, dim3((unsigned)(8 * per)), dim3(256), 0, s, (const uint8_t*)a.q, a.qs, a.m,
+                     a.codes, a.scales, a.n, a.nkb, a.out, mt, nt, per, std::max(4, 32 / a.nkb));
+  return TT_OK;
+}
+}  // namespace tt
+
+extern "C" {
 
 int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int32_t d, const uint8_t* codes,
                       const uint8_t* scales, int64_t n, void* out, int32_t out_dtype, void* ws, int64_t ws_bytes,
@@ -179,24 +227,35 @@ int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int3
   if (!cat_sizes_ok(m, d) || !cat_sizes_ok(n, d) || !dtype_ok(dtype) || !dtype_ok(out_dtype) || (m > 1 && ldq < d))
     return TT_ERR_ARG;
   if (m == 0 || n == 0) return TT_OK;
-  if (!q || !codes || !scales || !out || !ws) return TT_ERR_ARG;
-  if (ws_bytes < tt_cat_scores_workspace_bytes(m, n, d)) return TT_ERR_WORKSPACE;
-  const int nkb = cat_blocks(d);
-  const int64_t nt = (n + 63) / 64, mt = (m + 63) / 64;
-  if (mt > INT32_MAX / nt) return TT_ERR_UNSUPPORTED;
+  const int64_t need = tt_cat_scores_workspace_bytes(m, n, d);
+  if (!q || !codes || !scales || !out || (need > 0 && !ws)) return TT_ERR_ARG;
+  if (ws_bytes < need) return TT_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  uint8_t* qc = (uint8_t*)ws;
-  uint8_t* qs = qc + m * nkb * TT_BLOCK;
-  const CatRows r{nullptr, 0, m};
-  with_dtype(dtype, [&](auto t) {
-    hipLaunchKernelGGL(k_cat_write<decltype(t)::value>, dim3(grid_for(m * nkb, 16, 16384)), dim3(256), 0, s, q, m, ldq,
-                       d, nkb, r, qc, qs, (int32_t*)nullptr);
-  });
-  with_dtype(out_dtype, [&](auto t) {
-    hipLaunchKernelGGL(k_cat_scores<decltype(t)::value>, dim3((unsigned)(mt * nt)), dim3(256), 0, s, qc, qs, m, codes,
-                       scales, n, nkb, out, nt);
-  });
-  return ops_launch_check();
+  StreamArgs a{};
+  a.q = q;
+  a.codes = codes;
+  a.scales = scales;
+  a.out = out;
+  a.m = m;
+  a.n = n;
+  a.ldq = ldq;
+  a.d = d;
+  a.nkb = cat_blocks(d);
+  a.q_dtype = dtype;
+  if (need > 0) {
+    uint8_t* qc = (uint8_t*)ws;
+    uint8_t* qs = qc + m * a.nkb * TT_BLOCK;
+    const CatRows r{nullptr, 0, m};
+    with_dtype(dtype, [&](auto t) {
+      hipLaunchKernelGGL(k_cat_write<decltype(t)::value>, dim3(grid_for(m * a.nkb, 16, 16384)), dim3(256), 0, s, q, m,
+                         ldq, d, a.nkb, r, qc, qs, (int32_t*)nullptr);
+    });
+    a.q = qc;
+    a.qs = qs;
+  }
+  int rc = TT_OK;
+  with_dtype(out_dtype, [&](auto t) { rc = launch_scores<decltype(t)::value>(a, s); });
+  return rc ? rc : ops_launch_check();
 }
 
 int64_t tt_cat_dq_workspace_bytes(int64_t m, int64_t n, int32_t d) {
