@@ -483,9 +483,9 @@ __global__ __launch_bounds__(256, DT == TT_F32 ? 3 : 4) void k_cat_scores(
 }
 
 // ---------------------------------------------------------------------------
-// dq = dS C^: C^ is exact in bf16, dS is split into bf16 planes that hold it
-// exactly (bf16: 1, fp16: 2, fp32: 3), each plane product is exact in the
-// fp32 accumulator.  One wave: 16 rows of dS x 16 columns of dq.
+// dq = dS C^ on v_mfma_f32_16x16x32_bf16: C^ is exact in bf16, dS is split into
+// bf16 planes that hold it exactly (bf16: 1, fp16: 2, fp32: 3), each product
+// is exact in the fp32 accumulator.
 // ---------------------------------------------------------------------------
 // x as the sum of PL bf16 values: cut off, not rounded, so that each plane
 // holds the next 8 significant bits and nothing overflows; infinities and NaN
@@ -519,37 +519,225 @@ __device__ __forceinline__ void split_planes(const float (&x)[8], bf16x8 (&pl)[P
   for (int q = 0; q < PL; ++q) pl[q] = __builtin_bit_cast(bf16x8, w[q]);
 }
 
-template <int DT, int DQ>
-__global__ __launch_bounds__(64) void k_cat_dq(const void* ds, int64_t m, int64_t lds, int64_t n, const uint8_t* codes,
-                                               const uint8_t* scales, int d, int nkb, void* dq, int col_tiles) {
+struct DqArgs {
+  const void* ds;
+  int64_t m, lds, n;
+  const uint8_t *codes, *scales;
+  int d, nkb;
+  void* out;               // dq, or the parts [splits][m][d] in fp32
+  int64_t mt, splits, per; // row blocks, parts of the catalogue, workgroups of an XCD
+  int groups;              // column groups of 16 CT
+  int64_t part_steps;      // steps of DQ_STEP catalogue rows in a part
+};
+
+// 8 consecutive values of a row of dS as they lie in memory
+template <int DT> struct DsFrag {
+  u32x4 v[DT == TT_F32 ? 2 : 1];
+};
+template <int DT, bool MASK>
+__device__ __forceinline__ DsFrag<DT> load_ds(const void* row, int64_t at, int live) {
+  constexpr int ES = b8::Elem<DT>::SIZE;
+  DsFrag<DT> f;
+  const uint8_t* p = (const uint8_t*)row + at * ES;
+  if constexpr (!MASK) {
+    __builtin_memcpy(&f, p, 8 * ES);
+  } else {
+#pragma unroll
+    for (int w = 0; w < 2 * ES; ++w) {
+      uint32_t x = 0;
+      if constexpr (ES == 4) {
+        if (w < live) __builtin_memcpy(&x, p + 4 * w, 4);
+      } else {
+        uint16_t lo = 0, hi = 0;
+        if (2 * w < live) __builtin_memcpy(&lo, p + 4 * w, 2);
+        if (2 * w + 1 < live) __builtin_memcpy(&hi, p + 4 * w + 2, 2);
+        x = lo | (uint32_t)hi << 16;
+      }
+      f.v[w / 4][w % 4] = x;
+    }
+  }
+  return f;
+}
+template <int DT, int PL>
+__device__ __forceinline__ void ds_planes(const DsFrag<DT>& f, bf16x8 (&a)[PL]) {
+  if constexpr (DT == TT_BF16) {
+    a[0] = __builtin_bit_cast(bf16x8, f.v[0]);
+  } else {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      x[e] = DT == TT_F32 ? __uint_as_float(f.v[e / 4][e % 4])
+                          : b8::half_bits_to_float((uint16_t)(f.v[0][e / 2] >> (16 * (e & 1))));
+    split_planes<PL>(x, a);
+  }
+}
+
+// One workgroup: 16 RT WM rows of dS against a part of the catalogue, 16 CT
+// columns of dq in its waves' accumulators.  A step of DQ_STEP catalogue rows
+// is decoded once into LDS as bf16 [row][column] and read back transposed; the
+// next step's codes and dS values are on their way meanwhile.  WM waves take
+// different rows; with WM = 1 (up to 16 rows) the four share the rows and take
+// different thirty-twos of a step's catalogue rows, and add up at the end.
+constexpr int DQ_ROW_PAD = 32;  // bytes: 4 rows of a transposed read in distinct banks
+template <int WM> constexpr int DQ_STEP = WM == 1 ? 128 : 64;
+template <int CT, int WM> constexpr int dq_lds() {
+  const int stage = 2 * DQ_STEP<WM> * (32 * CT + DQ_ROW_PAD), sum = WM == 1 ? 4 * 16 * 16 * CT * 4 : 0;
+  return stage > sum ? stage : sum;
+}
+template <int DT, int DQ, int CT, int RT, int WM>
+__global__ __launch_bounds__(256, 2) void k_cat_dq(DqArgs a) {
   using namespace b8;
   constexpr int PL = DT == TT_BF16 ? 1 : DT == TT_F16 ? 2 : 3;
-  const int l = lane_id(), r = l & 15, g = l >> 4;
-  const int64_t m0 = (int64_t)(blockIdx.x / col_tiles) * 16;
-  const int c0 = (int)(blockIdx.x % col_tiles) * 16;
-  const int64_t row = min(m0 + r, m - 1);
-  f32x4 acc = zero4();
-  for (int64_t n0 = 0; n0 < n; n0 += 32) {
-    float x[8], c[8];
-    const int64_t nn = n0 + 8 * g;
-    ld8n<DT>(ds, row * lds + nn, (int)max((int64_t)0, min((int64_t)8, n - nn)), x);
+  constexpr int STEP = DQ_STEP<WM>, KS = WM == 1 ? 1 : 2;  // 32-row products of a wave in a step
+  constexpr int RS = 32 * CT + DQ_ROW_PAD;                 // bytes of a row in LDS
+  constexpr int CH = STEP * CT / 256;                      // 16-code pieces a thread decodes in a step
+  extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+  const int l = lane_id(), w = wave_id(), r = l & 15, g = l >> 4;
+  const int64_t id = (int64_t)(blockIdx.x & 7) * a.per + (blockIdx.x >> 3);
+  const int64_t row_blocks = a.mt * a.groups;
+  if (id >= row_blocks * a.splits) return;
+  const int64_t part = id / row_blocks, in = id % row_blocks;
+  const int col0 = (int)(in % a.groups) * 16 * CT;
+  const int64_t m0 = (in / a.groups) * (16 * RT * WM) + (WM == 1 ? 0 : w * 16 * RT);
+  const int64_t n = a.n, n_from = part * a.part_steps * STEP, n_to = min(n, n_from + a.part_steps * STEP);
+  const int64_t kp = (int64_t)a.nkb * ROWB;
+
+  const uint8_t* row[RT];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t cr = min(nn + e, n - 1);
-      float v[4];
-      decode4((uint32_t)codes[(cr * nkb) * BLK + c0 + r], scale_of(scales[cr * nkb + c0 / BLK]), v);
-      c[e] = nn + e < n ? v[0] : 0.f;
+  for (int i = 0; i < RT; ++i) row[i] = (const uint8_t*)a.ds + min(m0 + 16 * i + r, a.m - 1) * a.lds * Elem<DT>::SIZE;
+  const int ks0 = WM == 1 ? w : 0;  // this wave's first 32 rows of a step
+
+  u32x4 code[CH];
+  uint32_t byte[CH];
+  DsFrag<DT> ds[2][RT][KS];
+  auto fetch = [&](int64_t n0, DsFrag<DT> (&to)[RT][KS]) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int u = c * 256 + (int)threadIdx.x, cr = u / CT, cc = col0 + (u % CT) * 16;
+      const bool live = n0 + cr < n && cc < kp;
+      const int64_t at = min(n0 + cr, n - 1);
+      const int col = min(cc, (int)kp - 16);
+      __builtin_memcpy(&code[c], a.codes + at * kp + col, 16);
+      byte[c] = a.scales[at * a.nkb + col / ROWB];
+      if (!live) code[c] = (u32x4){0u, 0u, 0u, 0u}, byte[c] = 127u;
     }
-    bf16x8 a[PL], b[1];
-    split_planes<PL>(x, a);
-    split_planes<1>(c, b);
+    if (n0 + STEP <= n) {
 #pragma unroll
-    for (int q = PL - 1; q >= 0; --q) acc = mfma_bf16(a[q], b[0], acc);
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) to[i][k] = load_ds<DT, false>(row[i], n0 + 32 * (ks0 + k) + 8 * g, 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const int64_t at = n0 + 32 * (ks0 + k) + 8 * g;
+          to[i][k] = load_ds<DT, true>(row[i], at, (int)max((int64_t)0, min((int64_t)8, n - at)));
+        }
+    }
+  };
+  auto decode = [&](uint8_t* to) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int u = c * 256 + (int)threadIdx.x, cr = u / CT, cc = (u % CT) * 16;
+      const float s = scale_of(byte[c]);
+      *reinterpret_cast<bf16x8*>(to + cr * RS + cc * 2) = codes_to_bf16(code[c][0], code[c][1], s);
+      *reinterpret_cast<bf16x8*>(to + cr * RS + cc * 2 + 16) = codes_to_bf16(code[c][2], code[c][3], s);
+    }
+  };
+  f32x4 acc[RT][CT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[i][c] = zero4();
+  auto multiply = [&](const uint8_t* from, const DsFrag<DT> (&x)[RT][KS]) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      bf16x8 f[RT][PL];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) ds_planes<DT, PL>(x[i][k], f[i]);
+      const uint8_t* at = from + (32 * (ks0 + k) + 8 * g + (r >> 2)) * RS + (r & 3) * 8;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const bf16x8 b = tr_frag(reinterpret_cast<const uint16_t*>(at + 32 * c),
+                                 reinterpret_cast<const uint16_t*>(at + 32 * c + 4 * RS));
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int q = PL - 1; q >= 0; --q) acc[i][c] = mfma_bf16(f[i][q], b, acc[i][c]);
+      }
+    }
+  };
+
+  uint8_t* const stage[2] = {lds, lds + STEP * RS};
+  if (n_from < n_to) {
+    fetch(n_from, ds[0]);
+    decode(stage[0]);
   }
+  for (int64_t n0 = n_from; n0 < n_to; n0 += 2 * STEP) {
+    // two steps a round, so that each buffer has a name
+    __syncthreads();
+    const bool second = n0 + STEP < n_to;
+    if (second) fetch(n0 + STEP, ds[1]);
+    multiply(stage[0], ds[0]);
+    if (!second) break;
+    decode(stage[1]);
+    __syncthreads();
+    const bool third = n0 + 2 * STEP < n_to;
+    if (third) fetch(n0 + 2 * STEP, ds[0]);
+    multiply(stage[1], ds[1]);
+    if (third) decode(stage[0]);
+  }
+
+  if constexpr (WM == 1) {  // the four waves' sums, in wave order
+    __syncthreads();
+    float* const sum = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t i = m0 + 4 * g + e;
-    if (i < m && c0 + r < d) st1<DQ>(dq, i * d + c0 + r, acc[e]);
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[((w * 16 + 4 * g + e) * CT + c) * 16 + r] = acc[0][c][e];
+    __syncthreads();
+    constexpr int W = 16 * 16 * CT;
+    for (int u = (int)threadIdx.x; u < W; u += 256) {
+      const float v = ((sum[u] + sum[W + u]) + sum[2 * W + u]) + sum[3 * W + u];
+      const int i = u / (16 * CT), col = col0 + u % (16 * CT);
+      if (m0 + i < a.m && col < a.d) st1<DQ>(a.out, (part * a.m + m0 + i) * a.d + col, v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t at = m0 + 16 * i + 4 * g + e;
+          const int col = col0 + 16 * c + r;
+          if (at < a.m && col < a.d) st1<DQ>(a.out, (part * a.m + at) * a.d + col, acc[i][c][e]);
+        }
+  }
+}
+
+// dq = the parts' sum, in the parts' order within 16 interleaved chains (a tree
+// that the number of parts alone decides): 16 threads of 4 values a chain
+template <int DQ>
+__global__ __launch_bounds__(256) void k_cat_dq_sum(const float* part, int64_t parts, int64_t values, void* out) {
+  using namespace b8;
+  __shared__ float chain[16][64];
+  const int e = (int)threadIdx.x & 63, q = (int)threadIdx.x >> 6;  // 4 waves: chains q, q + 4, ...
+  const int64_t i = (int64_t)blockIdx.x * 64 + e;
+#pragma unroll
+  for (int c = q; c < 16; c += 4) {
+    float v = 0.f;
+    if (i < values)
+      for (int64_t s = c; s < parts; s += 16) v += part[s * values + i];
+    chain[c][e] = v;
+  }
+  __syncthreads();
+  if (q == 0 && i < values) {
+    float v = chain[0][e];
+#pragma unroll
+    for (int c = 1; c < 16; ++c) v += chain[c][e];
+    st1<DQ>(out, i, v);
   }
 }
 

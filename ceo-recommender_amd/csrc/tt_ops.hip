@@ -258,9 +258,67 @@ int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int3
   return rc ? rc : ops_launch_check();
 }
 
+}  // extern "C"
+
+namespace tt {
+// How dq's rows, columns and sum are split.  Parts of the catalogue until about
+// two workgroups a CU have work, none shorter than 8 steps; a part writes m d
+// floats and reads its share of the codes and of dS.
+struct DqPlan {
+  int ct, rt, wm, groups;
+  int64_t mt, splits, part_steps;
+};
+static DqPlan dq_plan(int64_t m, int64_t n, int32_t d) {
+  DqPlan p;
+  p.ct = d <= 64 ? 4 : d <= 128 ? 8 : 16;
+  p.wm = m <= 16 ? 1 : 4;
+  p.rt = m <= 64 || p.ct == 16 ? 1 : 2;  // 16 column tiles of two row tiles do not fit the registers
+  p.groups = (d + 16 * p.ct - 1) / (16 * p.ct);
+  p.mt = (m + 16 * p.rt * p.wm - 1) / (16 * p.rt * p.wm);
+  const int64_t step = p.wm == 1 ? 128 : 64, steps = std::max<int64_t>(1, (n + step - 1) / step);
+  const int64_t blocks = p.mt * p.groups;
+  int64_t s = std::max<int64_t>(1, std::min<int64_t>((512 + blocks - 1) / blocks, steps / 8));
+  p.part_steps = (steps + s - 1) / s;
+  p.splits = (steps + p.part_steps - 1) / p.part_steps;
+  return p;
+}
+
+template <int DT, int DQ, int CT, int RT, int WM>
+static void launch_dq_one(const DqArgs& a, hipStream_t s) {
+  constexpr int LDS = dq_lds<CT, WM>();
+  static std::once_flag once;
+  std::call_once(once, [] {
+    (void)hipFuncSetAttribute((const void*)k_cat_dq<DT, DQ, CT, RT, WM>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  });
+  hipLaunchKernelGGL((k_cat_dq<DT, DQ, CT, RT, WM>), dim3((unsigned)(8 * a.per)), dim3(256), LDS, s, a);
+}
+template <int DT, int DQ, int CT>
+static void launch_dq_rows(const DqArgs& a, const DqPlan& p, hipStream_t s) {
+  if (p.wm == 1)
+    launch_dq_one<DT, DQ, CT, 1, 1>(a, s);
+  else if (p.rt == 1)
+    launch_dq_one<DT, DQ, CT, 1, 4>(a, s);
+  else if constexpr (CT < 16)
+    launch_dq_one<DT, DQ, CT, 2, 4>(a, s);
+}
+template <int DT, int DQ>
+static void launch_dq(const DqArgs& a, const DqPlan& p, hipStream_t s) {
+  if (p.ct == 4)
+    launch_dq_rows<DT, DQ, 4>(a, p, s);
+  else if (p.ct == 8)
+    launch_dq_rows<DT, DQ, 8>(a, p, s);
+  else
+    launch_dq_rows<DT, DQ, 16>(a, p, s);
+}
+}  // namespace tt
+
+extern "C" {
+
 int64_t tt_cat_dq_workspace_bytes(int64_t m, int64_t n, int32_t d) {
   if (!cat_sizes_ok(m, d) || !cat_sizes_ok(n, d)) return TT_ERR_ARG;
-  return 0;
+  if (m == 0) return 0;
+  const DqPlan p = dq_plan(m, n, d);
+  return p.splits > 1 ? p.splits * m * d * (int64_t)sizeof(float) : 0;
 }
 
 int32_t tt_cat_dq(const void* ds, int32_t ds_dtype, int64_t m, int64_t lds, int64_t n, const uint8_t* codes,
@@ -272,15 +330,39 @@ int32_t tt_cat_dq(const void* ds, int32_t ds_dtype, int64_t m, int64_t lds, int6
   if (!dq || (n > 0 && (!ds || !codes || !scales))) return TT_ERR_ARG;
   const int64_t need = tt_cat_dq_workspace_bytes(m, n, d);
   if (need > 0 && (!ws || ws_bytes < need)) return TT_ERR_WORKSPACE;
-  const int nkb = cat_blocks(d), ct = (d + 15) / 16;
-  const int64_t mt = (m + 15) / 16;
-  if (mt > INT32_MAX / ct) return TT_ERR_UNSUPPORTED;
+  const DqPlan p = dq_plan(m, n, d);
+  if (p.mt > INT32_MAX / 16 / p.groups / p.splits) return TT_ERR_UNSUPPORTED;
+  hipStream_t s = (hipStream_t)stream;
+  DqArgs a;
+  a.ds = ds;
+  a.m = m;
+  a.lds = lds;
+  a.n = n;
+  a.codes = codes;
+  a.scales = scales;
+  a.d = d;
+  a.nkb = cat_blocks(d);
+  a.out = p.splits > 1 ? ws : dq;
+  a.mt = p.mt;
+  a.splits = p.splits;
+  a.per = (p.mt * p.groups * p.splits + 7) / 8;
+  a.groups = p.groups;
+  a.part_steps = p.part_steps;
   with_dtype(ds_dtype, [&](auto t) {
-    with_dtype(dq_dtype, [&](auto u) {
-      hipLaunchKernelGGL((k_cat_dq<decltype(t)::value, decltype(u)::value>), dim3((unsigned)(mt * ct)), dim3(64), 0,
-                         (hipStream_t)stream, ds, m, lds, n, codes, scales, d, nkb, dq, ct);
-    });
+    constexpr int DT = decltype(t)::value;
+    if (p.splits > 1)
+      launch_dq<DT, TT_F32>(a, p, s);
+    else
+      with_dtype(dq_dtype, [&](auto u) { launch_dq<DT, decltype(u)::value>(a, p, s); });
   });
+  if (p.splits > 1) {
+    const int64_t values = m * d;
+    if ((values + 63) / 64 > INT32_MAX) return TT_ERR_UNSUPPORTED;
+    with_dtype(dq_dtype, [&](auto u) {
+      hipLaunchKernelGGL(k_cat_dq_sum<decltype(u)::value>, dim3((unsigned)((values + 63) / 64)), dim3(256), 0, s,
+                         (const float*)ws, p.splits, values, dq);
+    });
+  }
   return ops_launch_check();
 }
 
