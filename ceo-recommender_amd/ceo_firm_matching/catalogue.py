@@ -46,49 +46,58 @@ def _rows_2d(x: torch.Tensor, d: int, what: str) -> torch.Tensor:
     return x
 
 
+def _scores(q, codes, scales, d, n, out_dtype):
+    """q [m, d] against the first n rows, [m, n] in out_dtype."""
+    dev = q.device
+    if dev.type != "cuda":
+        qv = block8.decode(*block8.encode(q), d)
+        return (qv @ block8.decode(codes[:n], scales[:n], d).t()).to(out_dtype)
+    m, L = q.shape[0], N.lib()
+    with N.on_device(dev):
+        out = torch.empty(m, n, dtype=out_dtype, device=dev)
+        wsb = L.tt_cat_scores_workspace_bytes(m, n, d)
+        if wsb < 0:
+            N.check(wsb, "tt_cat_scores_workspace_bytes")
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+        N.check(L.tt_cat_scores(q.data_ptr(), N.DTYPES[q.dtype], m, q.stride(0), d, codes.data_ptr(),
+                                scales.data_ptr(), n, out.data_ptr(), N.DTYPES[out_dtype], N.ptr(ws), wsb,
+                                N.stream_ptr(dev)), "tt_cat_scores")
+    return out
+
+
+def _dq(ds, codes, scales, d, n, dtype):
+    """ds [m, n] times the first n rows, [m, d] in dtype."""
+    dev, m = ds.device, ds.shape[0]
+    if dev.type != "cuda":
+        return (ds.to(torch.float32) @ block8.decode(codes[:n], scales[:n], d)).to(dtype)
+    if (n > 1 and ds.stride(1) != 1) or (m > 1 and ds.stride(0) < n):
+        ds = ds.contiguous()
+    L = N.lib()
+    with N.on_device(dev):
+        dq = torch.empty(m, d, dtype=dtype, device=dev)
+        wsb = L.tt_cat_dq_workspace_bytes(m, n, d, N.DTYPES[ds.dtype])
+        if wsb < 0:
+            N.check(wsb, "tt_cat_dq_workspace_bytes")
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+        N.check(L.tt_cat_dq(ds.data_ptr(), N.DTYPES[ds.dtype], m, ds.stride(0), n, codes.data_ptr(),
+                            scales.data_ptr(), d, dq.data_ptr(), N.DTYPES[dtype], N.ptr(ws), wsb,
+                            N.stream_ptr(dev)), "tt_cat_dq")
+    return dq
+
+
 class _ScoresFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, codes, scales, d, n, out_dtype):
         ctx.save_for_backward(codes, scales)
         ctx.meta = (d, n, q.dtype)
-        m = q.shape[0]
-        if q.device.type != "cuda":
-            qv = block8.decode(*block8.encode(q), d)
-            return (qv @ block8.decode(codes[:n], scales[:n], d).t()).to(out_dtype)
-        out = torch.empty(m, n, dtype=out_dtype, device=q.device)
-        L = N.lib()
-        wsb = int(L.tt_cat_scores_workspace_bytes(m, n, d))
-        if wsb < 0:
-            N.check(wsb, "tt_cat_scores_workspace_bytes")
-        with torch.cuda.device(q.device):
-            ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
-            N.check(L.tt_cat_scores(q.data_ptr(), N.DTYPES[q.dtype], m, q.stride(0), d, codes.data_ptr(),
-                                    scales.data_ptr(), n, out.data_ptr(), N.DTYPES[out_dtype], ws.data_ptr(), wsb,
-                                    N.stream_ptr(q.device)), "tt_cat_scores")
-        return out
+        return _scores(q, codes, scales, d, n, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, ds):
         codes, scales = ctx.saved_tensors
         d, n, dtype = ctx.meta
-        m = ds.shape[0]
-        if ds.device.type != "cuda":
-            dq = ds.to(torch.float32) @ block8.decode(codes[:n], scales[:n], d)
-            return dq.to(dtype), None, None, None, None, None
-        if (n > 1 and ds.stride(1) != 1) or (m > 1 and ds.stride(0) < n):
-            ds = ds.contiguous()
-        dq = torch.empty(m, d, dtype=dtype, device=ds.device)
-        L = N.lib()
-        wsb = int(L.tt_cat_dq_workspace_bytes(m, n, d))
-        if wsb < 0:
-            N.check(wsb, "tt_cat_dq_workspace_bytes")
-        with torch.cuda.device(ds.device):
-            ws = torch.empty(wsb, dtype=torch.uint8, device=ds.device)
-            N.check(L.tt_cat_dq(ds.data_ptr(), N.DTYPES[ds.dtype], m, ds.stride(0), n, codes.data_ptr(),
-                                scales.data_ptr(), d, dq.data_ptr(), N.DTYPES[dtype], ws.data_ptr(), wsb,
-                                N.stream_ptr(ds.device)), "tt_cat_dq")
-        return dq, None, None, None, None, None
+        return _dq(ds, codes, scales, d, n, dtype), None, None, None, None, None
 
 
 class EmbeddingCatalogue:
@@ -145,6 +154,8 @@ class EmbeddingCatalogue:
             raise ValueError(f"{what}: rows on {rows.device}, the catalogue on {self.device}")
         if m >= 0 and rows.shape[0] != m:
             raise ValueError(f"{what}: {rows.shape[0]} row numbers for {m} rows")
+        if rows.dtype == torch.int64 and rows.is_contiguous():
+            return rows
         return rows.to(torch.int64).contiguous()
 
     def _check_range(self, start: int, m: int, what: str):
@@ -178,7 +189,7 @@ class EmbeddingCatalogue:
                 r, i = torch.tensor(list(last.keys())), torch.tensor(list(last.values()))
                 self.codes[r], self.scales[r] = codes[i], scales[i]
             return
-        with torch.cuda.device(self.device):
+        with N.on_device(self.device):
             N.check(N.lib().tt_cat_write(emb.data_ptr(), N.DTYPES[emb.dtype], m, emb.stride(0), self.dim, N.ptr(rows),
                                          start, self.codes.data_ptr(), self.scales.data_ptr(), self.capacity,
                                          N.ptr(self._owner), N.stream_ptr(self.device)), "tt_cat_write")
@@ -205,7 +216,7 @@ class EmbeddingCatalogue:
             out = torch.zeros(m, self.dim)
             out[ok] = block8.decode(self.codes[rows[ok]], self.scales[rows[ok]], self.dim)
             return out.to(dtype)
-        with torch.cuda.device(self.device):
+        with N.on_device(self.device):
             out = torch.empty(m, self.dim, dtype=dtype, device=self.device)
             N.check(N.lib().tt_cat_read(self.codes.data_ptr(), self.scales.data_ptr(), self.capacity, self.dim,
                                         N.ptr(rows), start, m, out.data_ptr(), N.DTYPES[dtype], self.dim,
@@ -226,6 +237,10 @@ class EmbeddingCatalogue:
             raise ValueError(f"scores: expected [..., {self.dim}], got {tuple(queries.shape)}")
         n = self.capacity if count is None else int(count)
         self._check_range(0, n, "scores")
-        q = _rows_2d(queries.reshape(-1, self.dim), self.dim, "scores")
-        s = _ScoresFn.apply(q, self.codes, self.scales, self.dim, n, dtype)
-        return s.reshape(*queries.shape[:-1], n)
+        flat = queries.dim() == 2
+        q = _rows_2d(queries if flat else queries.reshape(-1, self.dim), self.dim, "scores")
+        if q.requires_grad and torch.is_grad_enabled():
+            s = _ScoresFn.apply(q, self.codes, self.scales, self.dim, n, dtype)
+        else:
+            s = _scores(q, self.codes, self.scales, self.dim, n, dtype)
+        return s if flat else s.reshape(*queries.shape[:-1], n)

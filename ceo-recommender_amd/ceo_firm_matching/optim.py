@@ -28,6 +28,7 @@ class _Bucket:
     def __init__(self, params, bits, capturable):
         self.params = params
         self.device = params[0].device if params else torch.device("cpu")
+        self.index = -1 if self.device.type == "cpu" else self.device.index  # Tensor.get_device()
         self.numel = [p.numel() for p in params]
         nb = [block8.blocks_of(n) for n in self.numel]
         self.block0 = [0] * len(nb)
@@ -50,6 +51,7 @@ class _Bucket:
         self.table[:, 2] = self.numel
         self.table[:, 3] = self.block0
         self.table[:, 5] = [N.DTYPES[p.dtype] for p in params]
+        self.table_at = self.table.ctypes.data
         s = N.TTAdamWState()
         if dev.type == "cuda":
             for field, t in zip(("exp_avg", "exp_avg_sq") if bits == 32 else ("m_codes", "m_scales", "r_codes", "r_scales"),
@@ -146,43 +148,49 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for g, b in zip(self.param_groups, self._buckets):
-            if not b.params:
+            live, params, grads = None, b.params, [p.grad for p in b.params]
+            try:
+                dense = [x.is_contiguous() for x in grads]
+            except AttributeError:  # parameters without a gradient among them
+                live = [i for i, x in enumerate(grads) if x is not None]
+                params, grads = [params[i] for i in live], [grads[i] for i in live]
+                dense = [x.layout == torch.strided and x.is_contiguous() for x in grads]
+            except RuntimeError:
+                dense = [False]
+            if not params:
                 continue
-            live, grads = [], []
-            for i, p in enumerate(b.params):
-                gr = p.grad
-                if gr is None:
-                    continue
-                if p.numel() != b.numel[i] or p.device != b.device or not p.is_contiguous():
-                    raise RuntimeError("AdamW: a parameter changed its size, device or layout after the optimizer was made")
-                if gr.layout != torch.strided:
+            sizes = b.numel if live is None else [b.numel[i] for i in live]
+            if ([p.numel() for p in params] != sizes or {p.get_device() for p in params} != {b.index}
+                    or not all([p.is_contiguous() for p in params])):
+                raise RuntimeError("AdamW: a parameter changed its size, device or layout after the optimizer was made")
+            if not all(dense):
+                if any(x.layout != torch.strided for x in grads):
                     raise NotImplementedError("AdamW: sparse gradients are not supported")
-                live.append(i)
-                grads.append(gr if gr.is_contiguous() else gr.contiguous())
-            if live:
+                grads = [x.contiguous() for x in grads]
+            if b.device.type == "cuda":
+                self._step_hip(g, b, live, params, grads)
+            else:
                 self._check_hyper(g)
-                if b.device.type == "cuda":
-                    self._step_hip(g, b, live, grads)
-                else:
-                    self._step_cpu(g, b, live, grads)
+                self._step_cpu(g, b, range(len(params)) if live is None else live, grads)
         return loss
 
-    def _step_hip(self, g, b, live, grads):
-        with torch.cuda.device(b.device):
+    def _step_hip(self, g, b, live, params, grads):
+        with N.on_device(b.device):
             if not self._capturable and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: a captured step needs capturable=True (the step count would be frozen)")
-            every = len(live) == len(b.params)
-            params = b.params if every else [b.params[i] for i in live]
-            t = b.table if every else b.table[live]
+            t, at = (b.table, b.table_at) if live is None else (b.table[live], 0)
             t[:, 0] = [p.data_ptr() for p in params]
             t[:, 1] = [x.data_ptr() for x in grads]
             if self._capturable:
-                t[:, 4] = live
+                t[:, 4] = range(len(params)) if live is None else live
+            elif live is None:
+                b.host_steps += 1
+                t[:, 4] = b.host_steps
             else:
                 b.host_steps[live] += 1
                 t[:, 4] = b.host_steps[live]
             hp = N.TTAdamWHP(g["lr"], g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"])
-            N.check(N.lib().tt_adamw_step(t.ctypes.data, len(live), self._bits, ctypes.byref(b.native),
+            N.check(N.lib().tt_adamw_step(at or t.ctypes.data, len(params), self._bits, ctypes.byref(b.native),
                                           ctypes.byref(hp), self._seed, N.stream_ptr(b.device)), "tt_adamw_step")
         torch.autograd.graph.increment_version(params)
 
@@ -231,7 +239,7 @@ class AdamW(torch.optim.Optimizer):
         if b.device.type != "cuda":
             return (block8.held(mc, ms, block8.E4M3).to(torch.bfloat16),
                     block8.held(rc, rs, block8.E4M4).to(torch.bfloat16))
-        with torch.cuda.device(b.device):
+        with N.on_device(b.device):
             m = torch.empty(b.n_blocks, block8.BLOCK, dtype=torch.bfloat16, device=b.device)
             r = torch.empty_like(m)
             N.check(N.lib().tt_adamw_held(ctypes.byref(b.native), m.data_ptr(), r.data_ptr(), N.stream_ptr(b.device)),

@@ -51,6 +51,35 @@ __global__ __launch_bounds__(256) void k_cat_disown(CatRows r, int64_t m, int32_
   }
 }
 
+// Up to CAT_FEW rows in one launch: every workgroup holds all row numbers in LDS
+// and the 16 lanes of a block look for a later mention of theirs (2 us at 333
+// rows, where three launches took 11)
+constexpr int CAT_FEW = 1024;
+template <int DT>
+__global__ __launch_bounds__(256) void k_cat_write_few(const void* x, int m, int64_t ldx, int d, int nkb, CatRows r,
+                                                       uint8_t* codes, uint8_t* scales) {
+  using namespace b8;
+  __shared__ int64_t rows[CAT_FEW];
+  for (int i = (int)threadIdx.x; i < m; i += 256) rows[i] = r.rows[i];
+  __syncthreads();
+  const int u = (int)(blockIdx.x * 256 + threadIdx.x) / LANES, lane = (int)threadIdx.x % LANES;
+  if (u >= m * nkb) return;
+  const int i = u / nkb, kb = u % nkb;
+  const int64_t c = rows[i];
+  if (!cat_row_ok(r, c)) return;
+  bool later = false;
+  for (int j = i + 1 + lane; j < m; j += LANES) later |= rows[j] == c;
+  const uint64_t any = __ballot(later) >> (threadIdx.x & 48) & 0xFFFFu;
+  if (any) return;
+  const int k = kb * BLK + lane * 8;
+  float v[8];
+  ld8n<DT>(x, i * ldx + k, max(0, min(8, d - k)), v);
+  uint32_t byte;
+  const u32x2 w = encode8(v, byte);
+  __builtin_memcpy(codes + (c * nkb + kb) * BLK + lane * 8, &w, 8);
+  if (lane == 0) scales[c * nkb + kb] = (uint8_t)byte;
+}
+
 template <int DT>
 __global__ __launch_bounds__(256) void k_cat_read(const uint8_t* codes, const uint8_t* scales, CatRows r, int64_t m,
                                                   int d, int nkb, void* out, int64_t ldo) {
@@ -534,27 +563,62 @@ struct DqArgs {
 template <int DT> struct DsFrag {
   u32x4 v[DT == TT_F32 ? 2 : 1];
 };
-template <int DT, bool MASK>
-__device__ __forceinline__ DsFrag<DT> load_ds(const void* row, int64_t at, int live) {
+// The same as it was loaded.  ODD (16-bit values, rows an odd number of them
+// apart, the first on a 4-byte boundary): loads at 2-byte addresses run at half
+// the rate (428 against 245 us at 16384 x 32771 x 128), so a lane loads the 5
+// words that hold its 8 values and shifts later.  The words reach one value
+// past the 8 and, in odd rows, one before: both are in the array, since the
+// steps that load this way end before the row does.
+template <int DT, bool ODD> struct DsLoad {
+  u32x4 v[DT == TT_F32 ? 2 : 1];
+  uint32_t next;
+};
+template <int DT> struct DsLoad<DT, false> {
+  u32x4 v[DT == TT_F32 ? 2 : 1];
+};
+template <int DT, bool ODD>
+__device__ __forceinline__ void load_ds(const uint8_t* row, int64_t at, DsLoad<DT, ODD>& to) {
+  const uint8_t* p = row + at * b8::Elem<DT>::SIZE;
+  if constexpr (ODD) {
+    const bool half = ((uintptr_t)row & 2) != 0;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p - (half ? 2 : 0));
+    __builtin_memcpy(&to.v[0], w, 16);
+    to.next = w[half ? 4 : 3];
+  } else {
+    __builtin_memcpy(&to.v, p, sizeof(to.v));
+  }
+}
+template <int DT, bool ODD>
+__device__ __forceinline__ DsFrag<DT> ds_values(const DsLoad<DT, ODD>& x, bool half) {
+  DsFrag<DT> f;
+  if constexpr (ODD) {
+    const uint32_t sh = half ? 16u : 0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      f.v[0][k] = __builtin_amdgcn_alignbit(k < 3 ? x.v[0][k + 1] : x.next, x.v[0][k], sh);
+  } else {
+    __builtin_memcpy(&f, &x, sizeof(f));
+  }
+  return f;
+}
+// one by one, zeros from `live` on
+template <int DT>
+__device__ __forceinline__ DsFrag<DT> load_ds_last(const uint8_t* row, int64_t at, int live) {
   constexpr int ES = b8::Elem<DT>::SIZE;
   DsFrag<DT> f;
-  const uint8_t* p = (const uint8_t*)row + at * ES;
-  if constexpr (!MASK) {
-    __builtin_memcpy(&f, p, 8 * ES);
-  } else {
+  const uint8_t* p = row + at * ES;
 #pragma unroll
-    for (int w = 0; w < 2 * ES; ++w) {
-      uint32_t x = 0;
-      if constexpr (ES == 4) {
-        if (w < live) __builtin_memcpy(&x, p + 4 * w, 4);
-      } else {
-        uint16_t lo = 0, hi = 0;
-        if (2 * w < live) __builtin_memcpy(&lo, p + 4 * w, 2);
-        if (2 * w + 1 < live) __builtin_memcpy(&hi, p + 4 * w + 2, 2);
-        x = lo | (uint32_t)hi << 16;
-      }
-      f.v[w / 4][w % 4] = x;
+  for (int w = 0; w < 2 * ES; ++w) {
+    uint32_t x = 0;
+    if constexpr (ES == 4) {
+      if (w < live) __builtin_memcpy(&x, p + 4 * w, 4);
+    } else {
+      uint16_t lo = 0, hi = 0;
+      if (2 * w < live) __builtin_memcpy(&lo, p + 4 * w, 2);
+      if (2 * w + 1 < live) __builtin_memcpy(&hi, p + 4 * w + 2, 2);
+      x = lo | (uint32_t)hi << 16;
     }
+    f.v[w / 4][w % 4] = x;
   }
   return f;
 }
@@ -576,7 +640,7 @@ __device__ __forceinline__ void ds_planes(const DsFrag<DT>& f, bf16x8 (&a)[PL]) 
 // columns of dq in its waves' accumulators.  A step of DQ_STEP catalogue rows
 // is decoded once into LDS as bf16 [row][column] and read back transposed; the
 // next step's codes and dS values are on their way meanwhile.  WM waves take
-// different rows; with WM = 1 (up to 16 rows) the four share the rows and take
+// different rows; with WM = 1 (up to 16 rows) four share the rows and take
 // different thirty-twos of a step's catalogue rows, and add up at the end.
 constexpr int DQ_ROW_PAD = 32;  // bytes: 4 rows of a transposed read in distinct banks
 template <int WM> constexpr int DQ_STEP = WM == 1 ? 128 : 64;
@@ -584,11 +648,12 @@ template <int CT, int WM> constexpr int dq_lds() {
   const int stage = 2 * DQ_STEP<WM> * (32 * CT + DQ_ROW_PAD), sum = WM == 1 ? 4 * 16 * 16 * CT * 4 : 0;
   return stage > sum ? stage : sum;
 }
-template <int DT, int DQ, int CT, int RT, int WM>
+template <int DT, int DQ, int CT, int RT, int WM, bool ODD>
 __global__ __launch_bounds__(256, 2) void k_cat_dq(DqArgs a) {
   using namespace b8;
   constexpr int PL = DT == TT_BF16 ? 1 : DT == TT_F16 ? 2 : 3;
-  constexpr int STEP = DQ_STEP<WM>, KS = WM == 1 ? 1 : 2;  // 32-row products of a wave in a step
+  constexpr int STEP = DQ_STEP<WM>;
+  constexpr int KS = WM == 1 ? 1 : STEP / 32;  // 32-row products of a wave in a step
   constexpr int RS = 32 * CT + DQ_ROW_PAD;                 // bytes of a row in LDS
   constexpr int CH = STEP * CT / 256;                      // 16-code pieces a thread decodes in a step
   extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
@@ -607,42 +672,64 @@ __global__ __launch_bounds__(256, 2) void k_cat_dq(DqArgs a) {
   for (int i = 0; i < RT; ++i) row[i] = (const uint8_t*)a.ds + min(m0 + 16 * i + r, a.m - 1) * a.lds * Elem<DT>::SIZE;
   const int ks0 = WM == 1 ? w : 0;  // this wave's first 32 rows of a step
 
-  u32x4 code[CH];
-  uint32_t byte[CH];
-  DsFrag<DT> ds[2][RT][KS];
-  auto fetch = [&](int64_t n0, DsFrag<DT> (&to)[RT][KS]) {
+  // this thread's 16-code pieces of a step, as offsets from the step's first row
+  const uint8_t* const codes = a.codes + col0;
+  uint32_t co[CH], so[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int u = c * 256 + (int)threadIdx.x, cr = u / CT;
+    const int cc = min((u % CT) * 16, (int)kp - 16 - col0);  // past the row's end: any codes, the columns are not stored
+    co[c] = (uint32_t)(cr * kp + cc);
+    so[c] = (uint32_t)(cr * a.nkb + (col0 + cc) / ROWB);
+  }
+  struct Codes {
+    u32x4 v[CH];
+    uint32_t byte[CH];
+  };
+  Codes code[2];
+  DsLoad<DT, ODD> ds[2][RT][KS];
+  auto fetch_codes = [&](int64_t n0, Codes& to) {
+    const uint8_t* c0 = codes + n0 * kp;
+    const uint8_t* s0 = a.scales + n0 * a.nkb;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int u = c * 256 + (int)threadIdx.x, cr = u / CT, cc = col0 + (u % CT) * 16;
-      const bool live = n0 + cr < n && cc < kp;
-      const int64_t at = min(n0 + cr, n - 1);
-      const int col = min(cc, (int)kp - 16);
-      __builtin_memcpy(&code[c], a.codes + at * kp + col, 16);
-      byte[c] = a.scales[at * a.nkb + col / ROWB];
-      if (!live) code[c] = (u32x4){0u, 0u, 0u, 0u}, byte[c] = 127u;
-    }
-    if (n0 + STEP <= n) {
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int k = 0; k < KS; ++k) to[i][k] = load_ds<DT, false>(row[i], n0 + 32 * (ks0 + k) + 8 * g, 8);
-    } else {
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const int64_t at = n0 + 32 * (ks0 + k) + 8 * g;
-          to[i][k] = load_ds<DT, true>(row[i], at, (int)max((int64_t)0, min((int64_t)8, n - at)));
-        }
+      to.v[c] = *reinterpret_cast<const u32x4*>(c0 + co[c]);
+      to.byte[c] = s0[so[c]];
     }
   };
-  auto decode = [&](uint8_t* to) {
+  auto fetch_ds = [&](int64_t n0, DsLoad<DT, ODD> (&to)[RT][KS]) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) load_ds<DT, ODD>(row[i], n0 + 32 * (ks0 + k) + 8 * g, to[i][k]);
+  };
+  // the catalogue's last step, shorter than the others: zeros past the end
+  auto fetch_last = [&](int64_t n0, Codes& cd, DsFrag<DT> (&to)[RT][KS]) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const bool live = n0 + (c * 256 + (int)threadIdx.x) / CT < n;
+      cd.v[c] = (u32x4){0u, 0u, 0u, 0u};
+      cd.byte[c] = 127u;
+      if (live) {
+        cd.v[c] = *reinterpret_cast<const u32x4*>(codes + n0 * kp + co[c]);
+        cd.byte[c] = a.scales[n0 * a.nkb + so[c]];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int64_t at = n0 + 32 * (ks0 + k) + 8 * g;
+        to[i][k] = load_ds_last<DT>(row[i], at, (int)max((int64_t)0, min((int64_t)8, n - at)));
+      }
+  };
+  auto decode = [&](const Codes& cd, uint8_t* to) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int u = c * 256 + (int)threadIdx.x, cr = u / CT, cc = (u % CT) * 16;
-      const float s = scale_of(byte[c]);
-      *reinterpret_cast<bf16x8*>(to + cr * RS + cc * 2) = codes_to_bf16(code[c][0], code[c][1], s);
-      *reinterpret_cast<bf16x8*>(to + cr * RS + cc * 2 + 16) = codes_to_bf16(code[c][2], code[c][3], s);
+      const float s = scale_of(cd.byte[c]);
+      *reinterpret_cast<bf16x8*>(to + cr * RS + cc * 2) = codes_to_bf16(cd.v[c][0], cd.v[c][1], s);
+      *reinterpret_cast<bf16x8*>(to + cr * RS + cc * 2 + 16) = codes_to_bf16(cd.v[c][2], cd.v[c][3], s);
     }
   };
   f32x4 acc[RT][CT];
@@ -650,12 +737,12 @@ __global__ __launch_bounds__(256, 2) void k_cat_dq(DqArgs a) {
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[i][c] = zero4();
-  auto multiply = [&](const uint8_t* from, const DsFrag<DT> (&x)[RT][KS]) {
+  auto multiply = [&](const uint8_t* from, auto values) {
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       bf16x8 f[RT][PL];
 #pragma unroll
-      for (int i = 0; i < RT; ++i) ds_planes<DT, PL>(x[i][k], f[i]);
+      for (int i = 0; i < RT; ++i) ds_planes<DT, PL>(values(i, k), f[i]);
       const uint8_t* at = from + (32 * (ks0 + k) + 8 * g + (r >> 2)) * RS + (r & 3) * 8;
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
@@ -670,23 +757,44 @@ __global__ __launch_bounds__(256, 2) void k_cat_dq(DqArgs a) {
   };
 
   uint8_t* const stage[2] = {lds, lds + STEP * RS};
-  if (n_from < n_to) {
-    fetch(n_from, ds[0]);
-    decode(stage[0]);
+  auto use = [&](int p) {
+    multiply(stage[p], [&](int i, int k) { return ds_values<DT, ODD>(ds[p][i][k], ((uintptr_t)row[i] & 2) != 0); });
+  };
+  // steps that end inside the row (ODD: before its end)
+  const int64_t whole = n_from + max((int64_t)0, min(n_to, ODD ? n - 1 : n) - n_from) / STEP * STEP;
+  if (n_from < whole) {
+    // two steps a round, so that each buffer has a name.  A buffer is filled
+    // again right after its use: dS two steps ahead, codes three (past the
+    // part's end the last step is fetched again, unused)
+    const int64_t end = whole - STEP;
+    fetch_codes(n_from, code[0]);
+    fetch_codes(min(n_from + STEP, end), code[1]);
+    fetch_ds(n_from, ds[0]);
+    fetch_ds(min(n_from + STEP, end), ds[1]);
+    decode(code[0], stage[0]);
+    fetch_codes(min(n_from + 2 * STEP, end), code[0]);
+    for (int64_t n0 = n_from;; n0 += 2 * STEP) {
+      __syncthreads();
+      use(0);
+      if (n0 + STEP >= whole) break;
+      fetch_ds(min(n0 + 2 * STEP, end), ds[0]);
+      decode(code[1], stage[1]);
+      fetch_codes(min(n0 + 3 * STEP, end), code[1]);
+      __syncthreads();
+      use(1);
+      if (n0 + 2 * STEP >= whole) break;
+      fetch_ds(min(n0 + 3 * STEP, end), ds[1]);
+      decode(code[0], stage[0]);
+      fetch_codes(min(n0 + 4 * STEP, end), code[0]);
+    }
   }
-  for (int64_t n0 = n_from; n0 < n_to; n0 += 2 * STEP) {
-    // two steps a round, so that each buffer has a name
+  if (whole < n_to) {
+    DsFrag<DT> last[RT][KS];
     __syncthreads();
-    const bool second = n0 + STEP < n_to;
-    if (second) fetch(n0 + STEP, ds[1]);
-    multiply(stage[0], ds[0]);
-    if (!second) break;
-    decode(stage[1]);
+    fetch_last(whole, code[0], last);
+    decode(code[0], stage[0]);
     __syncthreads();
-    const bool third = n0 + 2 * STEP < n_to;
-    if (third) fetch(n0 + 2 * STEP, ds[0]);
-    multiply(stage[1], ds[1]);
-    if (third) decode(stage[0]);
+    multiply(stage[0], [&](int i, int k) { return last[i][k]; });
   }
 
   if constexpr (WM == 1) {  // the four waves' sums, in wave order
@@ -717,26 +825,43 @@ __global__ __launch_bounds__(256, 2) void k_cat_dq(DqArgs a) {
   }
 }
 
-// dq = the parts' sum, in the parts' order within 16 interleaved chains (a tree
-// that the number of parts alone decides): 16 threads of 4 values a chain
+// dq = the parts' sum, in an order that their number alone decides: one after
+// the other, or 16 interleaved chains added in turn where there are many
 template <int DQ>
-__global__ __launch_bounds__(256) void k_cat_dq_sum(const float* part, int64_t parts, int64_t values, void* out) {
+__global__ __launch_bounds__(256) void k_cat_dq_sum_few(const float* part, int parts, int64_t values, void* out) {
   using namespace b8;
-  __shared__ float chain[16][64];
-  const int e = (int)threadIdx.x & 63, q = (int)threadIdx.x >> 6;  // 4 waves: chains q, q + 4, ...
-  const int64_t i = (int64_t)blockIdx.x * 64 + e;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= values) return;
+  if (i + 4 <= values && values % 4 == 0) {
+    f32x4 v = *reinterpret_cast<const f32x4*>(part + i);
+#pragma unroll 4
+    for (int s = 1; s < parts; ++s) v += *reinterpret_cast<const f32x4*>(part + s * values + i);
 #pragma unroll
-  for (int c = q; c < 16; c += 4) {
-    float v = 0.f;
-    if (i < values)
-      for (int64_t s = c; s < parts; s += 16) v += part[s * values + i];
-    chain[c][e] = v;
+    for (int e = 0; e < 4; ++e) st1<DQ>(out, i + e, v[e]);
+  } else {
+    for (int64_t k = i; k < min(i + 4, values); ++k) {
+      float v = part[k];
+      for (int s = 1; s < parts; ++s) v += part[s * values + k];
+      st1<DQ>(out, k, v);
+    }
   }
+}
+template <int DQ>
+__global__ __launch_bounds__(256) void k_cat_dq_sum(const float* part, int parts, int64_t values, void* out) {
+  using namespace b8;
+  __shared__ float chain[16][16];
+  const int e = (int)threadIdx.x & 15, c = (int)threadIdx.x >> 4;
+  const int64_t i = (int64_t)blockIdx.x * 16 + e;
+  float v = 0.f;
+  if (i < values) {
+#pragma unroll 8
+    for (int s = c; s < parts; s += 16) v += part[s * values + i];
+  }
+  chain[c][e] = v;
   __syncthreads();
-  if (q == 0 && i < values) {
-    float v = chain[0][e];
+  if (c == 0 && i < values) {
 #pragma unroll
-    for (int c = 1; c < 16; ++c) v += chain[c][e];
+    for (int q = 1; q < 16; ++q) v += chain[q][e];
     st1<DQ>(out, i, v);
   }
 }

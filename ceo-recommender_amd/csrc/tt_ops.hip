@@ -145,6 +145,13 @@ int32_t tt_cat_write(const void* x, int32_t dtype, int64_t m, int64_t ldx, int32
   hipStream_t s = (hipStream_t)stream;
   const CatRows r{rows, row0, capacity};
   const int nkb = cat_blocks(d);
+  if (rows && m <= CAT_FEW) {
+    with_dtype(dtype, [&](auto t) {
+      hipLaunchKernelGGL(k_cat_write_few<decltype(t)::value>, dim3(grid_for(m * nkb, 16, INT32_MAX)), dim3(256), 0, s, x,
+                         (int)m, ldx, d, nkb, r, codes, scales);
+    });
+    return ops_launch_check();
+  }
   if (rows) hipLaunchKernelGGL(k_cat_own, dim3(grid_for(m, 256, 4096)), dim3(256), 0, s, r, m, owner);
   with_dtype(dtype, [&](auto t) {
     hipLaunchKernelGGL(k_cat_write<decltype(t)::value>, dim3(grid_for(m * nkb, 16, 16384)), dim3(256), 0, s, x, m, ldx,
@@ -268,11 +275,11 @@ struct DqPlan {
   int ct, rt, wm, groups;
   int64_t mt, splits, part_steps;
 };
-static DqPlan dq_plan(int64_t m, int64_t n, int32_t d) {
+static DqPlan dq_plan(int64_t m, int64_t n, int32_t d, int32_t dtype) {
   DqPlan p;
   p.ct = d <= 64 ? 4 : d <= 128 ? 8 : 16;
   p.wm = m <= 16 ? 1 : 4;
-  p.rt = m <= 64 || p.ct == 16 ? 1 : 2;  // 16 column tiles of two row tiles do not fit the registers
+  p.rt = m <= 64 || (dtype == TT_F32 && p.ct == 16) ? 1 : 2;  // what the registers hold
   p.groups = (d + 16 * p.ct - 1) / (16 * p.ct);
   p.mt = (m + 16 * p.rt * p.wm - 1) / (16 * p.rt * p.wm);
   const int64_t step = p.wm == 1 ? 128 : 64, steps = std::max<int64_t>(1, (n + step - 1) / step);
@@ -283,14 +290,21 @@ static DqPlan dq_plan(int64_t m, int64_t n, int32_t d) {
   return p;
 }
 
-template <int DT, int DQ, int CT, int RT, int WM>
-static void launch_dq_one(const DqArgs& a, hipStream_t s) {
+template <int DT, int DQ, int CT, int RT, int WM, bool ODD>
+static void launch_dq_as(const DqArgs& a, hipStream_t s) {
   constexpr int LDS = dq_lds<CT, WM>();
   static std::once_flag once;
   std::call_once(once, [] {
-    (void)hipFuncSetAttribute((const void*)k_cat_dq<DT, DQ, CT, RT, WM>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    (void)hipFuncSetAttribute((const void*)k_cat_dq<DT, DQ, CT, RT, WM, ODD>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   });
-  hipLaunchKernelGGL((k_cat_dq<DT, DQ, CT, RT, WM>), dim3((unsigned)(8 * a.per)), dim3(256), LDS, s, a);
+  hipLaunchKernelGGL((k_cat_dq<DT, DQ, CT, RT, WM, ODD>), dim3((unsigned)(8 * a.per)), dim3(256), LDS, s, a);
+}
+template <int DT, int DQ, int CT, int RT, int WM>
+static void launch_dq_one(const DqArgs& a, hipStream_t s) {
+  if constexpr (DT != TT_F32) {
+    if (a.lds % 2 && (uintptr_t)a.ds % 4 == 0 && a.m > 1) return launch_dq_as<DT, DQ, CT, RT, WM, true>(a, s);
+  }
+  launch_dq_as<DT, DQ, CT, RT, WM, false>(a, s);
 }
 template <int DT, int DQ, int CT>
 static void launch_dq_rows(const DqArgs& a, const DqPlan& p, hipStream_t s) {
@@ -298,7 +312,7 @@ static void launch_dq_rows(const DqArgs& a, const DqPlan& p, hipStream_t s) {
     launch_dq_one<DT, DQ, CT, 1, 1>(a, s);
   else if (p.rt == 1)
     launch_dq_one<DT, DQ, CT, 1, 4>(a, s);
-  else if constexpr (CT < 16)
+  else if constexpr (!(DT == TT_F32 && CT == 16))
     launch_dq_one<DT, DQ, CT, 2, 4>(a, s);
 }
 template <int DT, int DQ>
@@ -314,10 +328,10 @@ static void launch_dq(const DqArgs& a, const DqPlan& p, hipStream_t s) {
 
 extern "C" {
 
-int64_t tt_cat_dq_workspace_bytes(int64_t m, int64_t n, int32_t d) {
-  if (!cat_sizes_ok(m, d) || !cat_sizes_ok(n, d)) return TT_ERR_ARG;
+int64_t tt_cat_dq_workspace_bytes(int64_t m, int64_t n, int32_t d, int32_t ds_dtype) {
+  if (!cat_sizes_ok(m, d) || !cat_sizes_ok(n, d) || !dtype_ok(ds_dtype)) return TT_ERR_ARG;
   if (m == 0) return 0;
-  const DqPlan p = dq_plan(m, n, d);
+  const DqPlan p = dq_plan(m, n, d, ds_dtype);
   return p.splits > 1 ? p.splits * m * d * (int64_t)sizeof(float) : 0;
 }
 
@@ -328,9 +342,9 @@ int32_t tt_cat_dq(const void* ds, int32_t ds_dtype, int64_t m, int64_t lds, int6
     return TT_ERR_ARG;
   if (m == 0) return TT_OK;
   if (!dq || (n > 0 && (!ds || !codes || !scales))) return TT_ERR_ARG;
-  const int64_t need = tt_cat_dq_workspace_bytes(m, n, d);
+  const int64_t need = tt_cat_dq_workspace_bytes(m, n, d, ds_dtype);
   if (need > 0 && (!ws || ws_bytes < need)) return TT_ERR_WORKSPACE;
-  const DqPlan p = dq_plan(m, n, d);
+  const DqPlan p = dq_plan(m, n, d, ds_dtype);
   if (p.mt > INT32_MAX / 16 / p.groups / p.splits) return TT_ERR_UNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
   DqArgs a;
@@ -357,10 +371,16 @@ int32_t tt_cat_dq(const void* ds, int32_t ds_dtype, int64_t m, int64_t lds, int6
   });
   if (p.splits > 1) {
     const int64_t values = m * d;
-    if ((values + 63) / 64 > INT32_MAX) return TT_ERR_UNSUPPORTED;
+    const bool few = p.splits <= 16;
+    const int64_t blocks = few ? (values + 1023) / 1024 : (values + 15) / 16;
+    if (blocks > INT32_MAX) return TT_ERR_UNSUPPORTED;
     with_dtype(dq_dtype, [&](auto u) {
-      hipLaunchKernelGGL(k_cat_dq_sum<decltype(u)::value>, dim3((unsigned)((values + 63) / 64)), dim3(256), 0, s,
-                         (const float*)ws, p.splits, values, dq);
+      if (few)
+        hipLaunchKernelGGL(k_cat_dq_sum_few<decltype(u)::value>, dim3((unsigned)blocks), dim3(256), 0, s,
+                           (const float*)ws, (int)p.splits, values, dq);
+      else
+        hipLaunchKernelGGL(k_cat_dq_sum<decltype(u)::value>, dim3((unsigned)blocks), dim3(256), 0, s, (const float*)ws,
+                           (int)p.splits, values, dq);
     });
   }
   return ops_launch_check();

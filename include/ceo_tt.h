@@ -546,8 +546,8 @@ int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int3
 /* dq [m, d] = dS C^ (the queries' rounding passes the gradient through; the
  * catalogue gets none).  ds [m, n] of ds_dtype with row stride lds; sums in
  * 32 bits, in an order that only the sizes decide.
- * ws: tt_cat_dq_workspace_bytes(m, n, d).                                   */
-int64_t tt_cat_dq_workspace_bytes(int64_t m, int64_t n, int32_t d);
+ * ws: tt_cat_dq_workspace_bytes(m, n, d, ds_dtype).                                   */
+int64_t tt_cat_dq_workspace_bytes(int64_t m, int64_t n, int32_t d, int32_t ds_dtype);
 int32_t tt_cat_dq(const void* ds, int32_t ds_dtype, int64_t m, int64_t lds, int64_t n,
                   const uint8_t* codes, const uint8_t* scales, int32_t d, void* dq,
                   int32_t dq_dtype, void* ws, int64_t ws_bytes, tt_stream_t stream);

@@ -48,14 +48,15 @@ int main() {
     for (int64_t n : {1, 100, 32771, 1000003})
       for (int32_t d : {1, 60, 128, 129, 512, 8192}) {
         CHECK(tt_cat_scores_workspace_bytes(m, n, d) >= 0);
-        CHECK(tt_cat_dq_workspace_bytes(m, n, d) >= 0);
+        CHECK(tt_cat_dq_workspace_bytes(m, n, d, 0) >= 0);
+        CHECK(tt_cat_dq_workspace_bytes(m, n, d, 1) >= 0);
         (void)tt_cat_scores(p, 0, m, d, d, b, b, n, p, 1, p, (int64_t)1 << 60, nullptr);
         (void)tt_cat_dq(p, 1, m, n, n, b, b, d, p, 1, p, (int64_t)1 << 60, nullptr);
       }
   CHECK(tt_cat_write(p, 0, 5, 8, 8, nullptr, 0, b, b, 4, nullptr, nullptr) == TT_ERR_ARG);
   CHECK(tt_cat_read(b, b, 4, 8, nullptr, 1, 4, p, 0, 8, nullptr) == TT_ERR_ARG);
   CHECK(tt_cat_scores_workspace_bytes(-1, 1, 1) == TT_ERR_ARG);
-  CHECK(tt_cat_dq_workspace_bytes(1, 1, 0) == TT_ERR_ARG);
+  CHECK(tt_cat_dq_workspace_bytes(1, 1, 0, 0) == TT_ERR_ARG);
   if (failures) {
     std::fprintf(stderr, "ops_host_check: %d FAILED\n", failures);
     return 1;

@@ -193,7 +193,7 @@ def test_host_argument_errors():
                dict(d=0), dict(m=-2), dict(n=-1)):
         assert scores(**kw) == N.TT_ERR_ARG, kw
     assert L.tt_cat_scores_workspace_bytes(-1, 4, 8) == N.TT_ERR_ARG
-    assert L.tt_cat_dq_workspace_bytes(4, 4, 0) == N.TT_ERR_ARG
+    assert L.tt_cat_dq_workspace_bytes(4, 4, 0, 0) == N.TT_ERR_ARG
 
     def dq(ds=p, dt=0, m=2, lds=4, n=4, codes=p, scales=p, d=8, out=p, odt=0, ws=p, wsb=1 << 30):
         return L.tt_cat_dq(ds, dt, m, lds, n, codes, scales, d, out, odt, ws, wsb, None)
