@@ -61,15 +61,27 @@ struct AdamwHp {
   float w1, b2, c2, eps, decay;
 };
 
-// p, m, v in; p', m', v' out; returns sqrt(v')
+// p, m, v in; p', m', v' out; returns sqrt(v').  FAST (8-bit states, whose
+// kernel the instructions bound): the hardware's square root and reciprocal,
+// off by one unit in the last place each, for the correctly rounded ones of
+// about 12 instructions.
+template <bool FAST>
 __device__ __forceinline__ float adamw_elem(float& p, float& m, float& v, float g, const AdamwHp& h,
-                                            const AdamwCoef& c) {
+                                            const AdamwCoef& c, float inv_bc2s) {
   m = m + h.w1 * (g - m);
   v = v * h.b2 + (h.c2 * g) * g;
+  if constexpr (FAST) {
+    const float r = __builtin_amdgcn_sqrtf(v);
+    p = p * h.decay - c.step_size * (m * __builtin_amdgcn_rcpf(r * inv_bc2s + h.eps));
+    return r;
+  }
   const float r = sqrtf(v);
   p = p * h.decay - c.step_size * (m / (r / c.bc2s + h.eps));
   return r;
 }
+
+// whether a byte of w is 0xFF (and at times where one is 0xFE below a 0xFF: never without one)
+__device__ __forceinline__ bool has_ff(uint32_t w) { return ((~w - 0x01010101u) & w & 0x80808080u) != 0; }
 
 template <int BITS, int DT>
 __device__ __forceinline__ void adamw_chunk(const AdamwArgs& a, int k, const AdamwCoef& c, int64_t from) {
@@ -79,6 +91,48 @@ __device__ __forceinline__ void adamw_chunk(const AdamwArgs& a, int k, const Ada
   const void* const G = a.g[k];
   const int64_t n = a.n[k], blk0 = a.blk[k];
   const int64_t to = min(from + (int64_t)a.chunk, n);
+  const float inv_bc2s = 1.f / c.bc2s;
+  if constexpr (BITS == 32) {
+    // 4 values a thread, twice: every access of a wave covers whole lines
+    constexpr int PER = 4, HALF = ADAMW_STRIDE / 2;
+    int64_t at = from;
+    for (; at + ADAMW_STRIDE <= to; at += ADAMW_STRIDE) {  // no tests between the loads
+      const int64_t i = at + (int64_t)threadIdx.x * PER;
+      float p[2][PER], g[2][PER], m[2][PER], v[2][PER];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        ldv<DT, PER>(P, i + q * HALF, p[q]);
+        ldv<DT, PER>(G, i + q * HALF, g[q]);
+        ldv<TT_F32, PER>(a.m, blk0 * BLK + i + q * HALF, m[q]);
+        ldv<TT_F32, PER>(a.v, blk0 * BLK + i + q * HALF, v[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) adamw_elem<false>(p[q][e], m[q][e], v[q][e], g[q][e], h, c, 0.f);
+        stv<DT, PER>(P, i + q * HALF, p[q]);
+        stv<TT_F32, PER>(a.m, blk0 * BLK + i + q * HALF, m[q]);
+        stv<TT_F32, PER>(a.v, blk0 * BLK + i + q * HALF, v[q]);
+      }
+    }
+    for (int64_t i = at + (int64_t)threadIdx.x * PER; i < to; i += HALF) {
+      const int live = (int)min((int64_t)PER, to - i);
+      float p[PER], g[PER], m[PER], v[PER];
+      ldn<DT, PER>(P, i, live, p);
+      ldn<DT, PER>(G, i, live, g);
+      ldn<TT_F32, PER>(a.m, blk0 * BLK + i, live, m);
+      ldn<TT_F32, PER>(a.v, blk0 * BLK + i, live, v);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) adamw_elem<false>(p[e], m[e], v[e], g[e], h, c, 0.f);
+      stn<DT, PER>(P, i, live, p);
+      stn<TT_F32, PER>(a.m, blk0 * BLK + i, live, m);  // (the padding stays zero)
+      stn<TT_F32, PER>(a.v, blk0 * BLK + i, live, v);
+    }
+    return;
+  }
+  uint32_t place[8];  // of the hash: this thread's values keep their places in their blocks
+#pragma unroll
+  for (int e = 0; e < 8; ++e) place[e] = (threadIdx.x % LANES * 8 + e) * 0x9E3779B9u;
   for (int64_t i = from + (int64_t)threadIdx.x * 8; i - (int64_t)(threadIdx.x % LANES) * 8 < to; i += ADAMW_STRIDE) {
     // the 16 lanes of a block stay together; lanes past the tensor's end see zeros
     const int live = (int)max((int64_t)0, min((int64_t)8, n - i));
@@ -86,54 +140,60 @@ __device__ __forceinline__ void adamw_chunk(const AdamwArgs& a, int k, const Ada
     float p[8], g[8], m[8], v[8];
     ld8n<DT>(P, i, live, p);
     ld8n<DT>(G, i, live, g);
-    if constexpr (BITS == 32) {
-      ld8<TT_F32>(a.m, s, m);
-      ld8<TT_F32>(a.v, s, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) adamw_elem(p[e], m[e], v[e], g[e], h, c);
-      if (live < 8)  // the padding stays zero
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e >= live) m[e] = v[e] = 0.f;
-      st8<TT_F32>(a.m, s, m);
-      st8<TT_F32>(a.v, s, v);
-    } else {
+    {
       const int64_t b = blk0 + (i / BLK);
       u32x2 mc, rc;
       __builtin_memcpy(&mc, a.mc + s, 8);
       __builtin_memcpy(&rc, a.rc + s, 8);
-      const float sm = scale_of(a.ms[b]), sr = scale_of(a.rs[b]);
-      float r[8];
+      const uint32_t bm = a.ms[b], br = a.rs[b];
+      decode8(mc, scale_of(bm), m);  // e4m3: the hardware's conversion, NaN and signs with it
+      float r[8], root[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) root[e] = code_value<MANT_R>((rc[e / 4] >> (8 * (e % 4))) & 0xFFu, br);
+      if (__ballot(has_ff(rc[0]) || has_ff(rc[1]))) {
+        asm volatile("");
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (((rc[e / 4] >> (8 * (e % 4))) & 0xFFu) == NAN_R) root[e] = __uint_as_float(0x7FC00000u);
+      }
       uint32_t am = 0, ar = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t cm = (mc[e / 4] >> (8 * (e % 4))) & 0xFFu, cr = (rc[e / 4] >> (8 * (e % 4))) & 0xFFu;
-        const float nan = __uint_as_float(0x7FC00000u);
-        const float mag = (cm & 0x7Fu) == NAN_M ? nan : code_value<MANT_M>(cm & 0x7Fu, sm);
-        m[e] = (cm & 0x80u) ? -mag : mag;
-        const float root = cr == NAN_R ? nan : code_value<MANT_R>(cr, sr);
-        v[e] = root * root;
-        r[e] = adamw_elem(p[e], m[e], v[e], g[e], h, c);
-        const uint32_t bm = __float_as_uint(m[e]) & 0x7FFFFFFFu, br = __float_as_uint(r[e]);
-        am = max(am, finite_bits(bm) ? bm : 0u);
-        ar = max(ar, finite_bits(br) ? br : 0u);  // a NaN's sign bit, too, is over the finite ones
+        v[e] = root[e] * root[e];
+        r[e] = adamw_elem<true>(p[e], m[e], v[e], g[e], h, c, inv_bc2s);
+        am = max(am, __float_as_uint(m[e]) & 0x7FFFFFFFu);
+        ar = max(ar, __float_as_uint(r[e]));  // a root's sign bit is a NaN's
+      }
+      const bool odd = !finite_bits(am) || !finite_bits(ar);
+      u32x2 nan_m = {0u, 0u}, nan_r = {0u, 0u};
+      if (__ballot(odd)) {  // infinities or NaN somewhere in the wave: held as NaN, the others by the finite ones
+        asm volatile("");    // a branch, not 40 selects
+        am = ar = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t xm = __float_as_uint(m[e]) & 0x7FFFFFFFu, xr = __float_as_uint(r[e]);
+          if (!finite_bits(xm)) m[e] = 0.f, nan_m[e / 4] |= NAN_M << (8 * (e % 4));
+          if (!finite_bits(xr)) r[e] = 0.f, nan_r[e / 4] |= NAN_R << (8 * (e % 4));
+          am = max(am, finite_bits(xm) ? xm : 0u);
+          ar = max(ar, finite_bits(xr) ? xr : 0u);
+        }
       }
       const uint32_t ym = (uint32_t)scale_byte(row_max16(am), CARRY_M);
       const uint32_t yr = (uint32_t)scale_byte(row_max16(ar), CARRY_R);
-      const float im = inv_scale(ym), ir = inv_scale(yr);
       const uint32_t rk = perm32((uint32_t)b ^ c.key_lo) + c.key_hi;
       mc = rc = (u32x2){0u, 0u};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t u = perm32(rk ^ ((uint32_t)((i % BLK) + e) * 0x9E3779B9u));
-        const uint32_t bm = __float_as_uint(m[e]);
-        uint32_t cm = finite_bits(bm & 0x7FFFFFFFu) ? round_code<MANT_M>(fabsf(m[e]) * im, u & 0xFFFFu) : NAN_M;
-        cm |= (bm >> 24) & 0x80u;
-        uint32_t cr = finite_bits(__float_as_uint(r[e])) ? round_code<MANT_R>(r[e] * ir, u >> 16) : NAN_R;
-        cr = r[e] > 0.f ? max(cr, 1u) : cr;  // a positive root stays positive: m' / sqrt(v') stays bounded
+        const uint32_t u = perm32(rk ^ place[e]);
+        const uint32_t xm = __float_as_uint(m[e]), xr = __float_as_uint(r[e]);
+        const uint32_t cm = round_code<MANT_M>(fabsf(m[e]), ym, u & 0xFFFFu) | (xm >> 24 & 0x80u);
+        // a positive root stays positive: m' / sqrt(v') stays bounded
+        const uint32_t cr = max(round_code<MANT_R>(r[e], yr, u >> 16), min(xr, 1u));
         mc[e / 4] |= cm << (8 * (e % 4));
         rc[e / 4] |= cr << (8 * (e % 4));
       }
+      mc |= nan_m;
+      rc |= nan_r;
       if (live < 8) {  // the padding stays zero
         const uint64_t keep = live > 0 ? ~0ull >> (64 - 8 * live) : 0ull;
         mc[0] &= (uint32_t)keep, mc[1] &= (uint32_t)(keep >> 32);
@@ -176,7 +236,7 @@ __global__ __launch_bounds__(256) void k_adamw_held(const uint8_t* mc, const uin
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += (int64_t)gridDim.x * blockDim.x) {
     u32x2 w;
     __builtin_memcpy(&w, codes + i * 8, 8);
-    const float s = scale_of(scales[i / LANES]);
+    const uint32_t s = scales[i / LANES];
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {

@@ -60,7 +60,7 @@ template <> struct Elem<TT_F16> {
   static constexpr int SIZE = 2;
 };
 
-// one value / 8 consecutive values.  Any address that the type's own
+// one value / N consecutive values.  Any address that the type's own
 // alignment allows: gfx950 does unaligned vector accesses in hardware.
 template <int DT>
 __device__ __forceinline__ float ld1(const void* p, int64_t i) {
@@ -75,48 +75,56 @@ __device__ __forceinline__ void st1(void* p, int64_t i, float v) {
   else
     reinterpret_cast<uint16_t*>(p)[i] = DT == TT_BF16 ? bf16_bits(v) : float_to_half_bits(v);
 }
-template <int DT>
-__device__ __forceinline__ void ld8(const void* p, int64_t i, float (&x)[8]) {
+template <int DT, int N>
+__device__ __forceinline__ void ldv(const void* p, int64_t i, float (&x)[N]) {
   if constexpr (DT == TT_F32) {
-    __builtin_memcpy(x, reinterpret_cast<const float*>(p) + i, 32);
+    __builtin_memcpy(x, reinterpret_cast<const float*>(p) + i, 4 * N);
   } else {
-    uint16_t h[8];
-    __builtin_memcpy(h, reinterpret_cast<const uint16_t*>(p) + i, 16);
+    uint16_t h[N];
+    __builtin_memcpy(h, reinterpret_cast<const uint16_t*>(p) + i, 2 * N);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = DT == TT_BF16 ? bf16_val(h[k]) : half_bits_to_float(h[k]);
+    for (int k = 0; k < N; ++k) x[k] = DT == TT_BF16 ? bf16_val(h[k]) : half_bits_to_float(h[k]);
   }
 }
-template <int DT>
-__device__ __forceinline__ void st8(void* p, int64_t i, const float (&x)[8]) {
+template <int DT, int N>
+__device__ __forceinline__ void stv(void* p, int64_t i, const float (&x)[N]) {
   if constexpr (DT == TT_F32) {
-    __builtin_memcpy(reinterpret_cast<float*>(p) + i, x, 32);
+    __builtin_memcpy(reinterpret_cast<float*>(p) + i, x, 4 * N);
   } else {
-    uint16_t h[8];
+    uint32_t h[N / 2];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) h[k] = DT == TT_BF16 ? bf16_bits(x[k]) : float_to_half_bits(x[k]);
-    __builtin_memcpy(reinterpret_cast<uint16_t*>(p) + i, h, 16);
+    for (int k = 0; k < N / 2; ++k)
+      h[k] = DT == TT_BF16 ? pk_bf16(x[2 * k], x[2 * k + 1])
+                           : float_to_half_bits(x[2 * k]) | (uint32_t)float_to_half_bits(x[2 * k + 1]) << 16;
+    __builtin_memcpy(reinterpret_cast<uint16_t*>(p) + i, h, 2 * N);
   }
 }
-// the first k (0..8) of 8 values; the rest read as zero, are not written
-template <int DT>
-__device__ __forceinline__ void ld8n(const void* p, int64_t i, int k, float (&x)[8]) {
-  if (k >= 8) {
-    ld8<DT>(p, i, x);
+// the first k (0..N) of N values; the rest read as zero, are not written
+template <int DT, int N>
+__device__ __forceinline__ void ldn(const void* p, int64_t i, int k, float (&x)[N]) {
+  if (k >= N) {
+    ldv<DT, N>(p, i, x);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < k ? ld1<DT>(p, i + j) : 0.f;
+    for (int j = 0; j < N; ++j) x[j] = j < k ? ld1<DT>(p, i + j) : 0.f;
   }
 }
-template <int DT>
-__device__ __forceinline__ void st8n(void* p, int64_t i, int k, const float (&x)[8]) {
-  if (k >= 8) {
-    st8<DT>(p, i, x);
+template <int DT, int N>
+__device__ __forceinline__ void stn(void* p, int64_t i, int k, const float (&x)[N]) {
+  if (k >= N) {
+    stv<DT, N>(p, i, x);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < N; ++j)
       if (j < k) st1<DT>(p, i + j, x[j]);
   }
 }
+template <int DT>
+__device__ __forceinline__ void ld8n(const void* p, int64_t i, int k, float (&x)[8]) { ldn<DT, 8>(p, i, k, x); }
+template <int DT>
+__device__ __forceinline__ void st8n(void* p, int64_t i, int k, const float (&x)[8]) { stn<DT, 8>(p, i, k, x); }
+template <int DT>
+__device__ __forceinline__ void st8(void* p, int64_t i, const float (&x)[8]) { stv<DT, 8>(p, i, x); }
 
 // ---- e4m3, rounded to nearest even (the catalogue) -------------------------
 // 8 values under a scale byte -> 8 code bytes; infinities become NaN: e4m3 has none
@@ -160,18 +168,19 @@ __device__ __forceinline__ void decode8(u32x2 c, float s, float (&x)[8]) {
 }
 
 // ---- magnitudes rounded up or down by 16 random bits (the states) ----------
-// The code of y >= 0 is y's own float bits after y * 2^-120 has moved the
-// code's exponent bias (7) to the float's: normal and subnormal codes alike
-// are then the top bits, what is cut off is the rest, and adding random bits
-// below the cut rounds up with the probability of what is cut.
+// The code of x >= 0 under a scale 2^(byte - 127) is x's own float bits after
+// x * 2^(127 - byte - 120) has moved the code's exponent bias (7) to the
+// float's: normal and subnormal codes alike are then the top bits, what is cut
+// off is the rest, and adding random bits below the cut rounds up with the
+// probability of what is cut.
 template <int MANT>
-__device__ __forceinline__ uint32_t round_code(float y, uint32_t rnd16) {
+__device__ __forceinline__ uint32_t round_code(float x, uint32_t byte, uint32_t rnd16) {
   constexpr int SH = 23 - MANT;
-  return (__float_as_uint(y * 0x1p-120f) + (rnd16 << (SH - 16))) >> SH;
+  return (__float_as_uint(__builtin_amdgcn_ldexpf(x, 7 - (int)byte)) + (rnd16 << (SH - 16))) >> SH;
 }
 template <int MANT>
-__device__ __forceinline__ float code_value(uint32_t mag, float s) {
-  return __uint_as_float(mag << (23 - MANT)) * 0x1p120f * s;
+__device__ __forceinline__ float code_value(uint32_t mag, uint32_t byte) {
+  return __builtin_amdgcn_ldexpf(__uint_as_float(mag << (23 - MANT)), (int)byte - 7);
 }
 
 }  // namespace b8

@@ -22,26 +22,33 @@ __global__ __launch_bounds__(256) void k_cat_own(CatRows r, int64_t m, int32_t* 
   }
 }
 
-// 16 lanes a block of 128: 8 values each
+// 16 lanes take up to CAT_UNIT blocks of a row (blockIdx.y: which ones), 8
+// values each: all loads first, one row number and one owner for all of them
+constexpr int CAT_UNIT = 2;
 template <int DT>
 __global__ __launch_bounds__(256) void k_cat_write(const void* x, int64_t m, int64_t ldx, int d, int nkb, CatRows r,
                                                    uint8_t* codes, uint8_t* scales, int32_t* owner) {
   using namespace b8;
-  const int64_t total = m * nkb;
-  for (int64_t u = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES; u < total;
-       u += (int64_t)gridDim.x * blockDim.x / LANES) {
-    const int64_t i = u / nkb;
-    const int kb = (int)(u - i * nkb);
+  const int lane = (int)threadIdx.x % LANES, kb0 = (int)blockIdx.y * CAT_UNIT;
+  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES; i < m;
+       i += (int64_t)gridDim.x * blockDim.x / LANES) {
     const int64_t c = cat_row(r, i);
     if (!cat_row_ok(r, c)) continue;
     if (owner && owner[c] != (int32_t)i + 1) continue;
-    const int k = kb * BLK + (int)(threadIdx.x % LANES) * 8;
-    float v[8];
-    ld8n<DT>(x, i * ldx + k, max(0, min(8, d - k)), v);
-    uint32_t byte;
-    const u32x2 w = encode8(v, byte);
-    __builtin_memcpy(codes + (c * nkb + kb) * BLK + (threadIdx.x % LANES) * 8, &w, 8);
-    if (threadIdx.x % LANES == 0) scales[c * nkb + kb] = (uint8_t)byte;
+    float v[CAT_UNIT][8];
+#pragma unroll
+    for (int b = 0; b < CAT_UNIT; ++b) {
+      const int k = (kb0 + b) * BLK + lane * 8;
+      ld8n<DT>(x, i * ldx + k, max(0, min(8, d - k)), v[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < CAT_UNIT; ++b)
+      if (kb0 + b < nkb) {
+        uint32_t byte;
+        const u32x2 w = encode8(v[b], byte);
+        __builtin_memcpy(codes + (c * nkb + kb0 + b) * BLK + lane * 8, &w, 8);
+        if (lane == 0) scales[c * nkb + kb0 + b] = (uint8_t)byte;
+      }
   }
 }
 __global__ __launch_bounds__(256) void k_cat_disown(CatRows r, int64_t m, int32_t* owner) {
@@ -84,20 +91,29 @@ template <int DT>
 __global__ __launch_bounds__(256) void k_cat_read(const uint8_t* codes, const uint8_t* scales, CatRows r, int64_t m,
                                                   int d, int nkb, void* out, int64_t ldo) {
   using namespace b8;
-  const int64_t total = m * nkb;
-  for (int64_t u = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES; u < total;
-       u += (int64_t)gridDim.x * blockDim.x / LANES) {
-    const int64_t i = u / nkb;
-    const int kb = (int)(u - i * nkb);
+  const int lane = (int)threadIdx.x % LANES, kb0 = (int)blockIdx.y * CAT_UNIT;
+  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / LANES; i < m;
+       i += (int64_t)gridDim.x * blockDim.x / LANES) {
     const int64_t c = cat_row(r, i);
-    const int k = kb * BLK + (int)(threadIdx.x % LANES) * 8;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (cat_row_ok(r, c)) {
-      u32x2 w;
-      __builtin_memcpy(&w, codes + (c * nkb + kb) * BLK + (threadIdx.x % LANES) * 8, 8);
-      decode8(w, scale_of(scales[c * nkb + kb]), v);
+    u32x2 w[CAT_UNIT];
+    uint32_t byte[CAT_UNIT];
+    const bool ok = cat_row_ok(r, c);
+#pragma unroll
+    for (int b = 0; b < CAT_UNIT; ++b) {
+      w[b] = (u32x2){0u, 0u};
+      byte[b] = 127u;
+      if (ok && kb0 + b < nkb) {
+        __builtin_memcpy(&w[b], codes + (c * nkb + kb0 + b) * BLK + lane * 8, 8);
+        byte[b] = scales[c * nkb + kb0 + b];
+      }
     }
-    st8n<DT>(out, i * ldo + k, max(0, min(8, d - k)), v);
+#pragma unroll
+    for (int b = 0; b < CAT_UNIT; ++b) {
+      const int k = (kb0 + b) * BLK + lane * 8;
+      float v[8];
+      decode8(w[b], scale_of(byte[b]), v);
+      st8n<DT>(out, i * ldo + k, max(0, min(8, d - k)), v);
+    }
   }
 }
 
@@ -243,41 +259,13 @@ struct StreamArgs {
   int64_t panels, strips, per;  // workgroup t of an XCD's share: panel t / strips, strip t % strips
 };
 
-// codes and scale byte of this lane's query in the block from k: values 16 g .. and 64 + 16 g ..
-template <int QDT>
-__device__ __forceinline__ i32x8 encode_query(const void* q, int64_t at, int k, int d, bool live, int& byte) {
-  using namespace b8;
-  float x[4][8];
-  uint32_t amax = 0;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int kc = k + 8 * (c & 1) + 64 * (c >> 1);
-    ld8n<QDT>(q, at + kc, live ? max(0, min(8, d - kc)) : 0, x[c]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t a = __float_as_uint(x[c][e]) & 0x7FFFFFFFu;
-      amax = max(amax, finite_bits(a) ? a : 0u);
-    }
-  }
-  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
-  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-  byte = scale_byte(amax, CARRY_M);
-  i32x8 w;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const u32x2 p = encode8_scaled(x[c], (uint32_t)byte);
-    w[2 * c] = (int)p[0];
-    w[2 * c + 1] = (int)p[1];
-  }
-  return w;
-}
-
 // NKB: blocks a row, 0: any number, with the queries' codes read again for every tile
 template <int DT, int IT, int QT, int NKB, bool ENC>
 __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs a) {
   using namespace b8;
   constexpr int KB = NKB ? NKB : 1;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * tile_lds<DT, IT, QT>()];
+  __shared__ __attribute__((aligned(16))) uint8_t enc[ENC ? 16 * KB * (ROWB + 1) : 16];  // ENC: the queries' codes, scale bytes
   const int l = lane_id(), w = wave_id(), r = l & 15, g = l >> 4;
   uint8_t* const so = lds + w * tile_lds<DT, IT, QT>();
   const int64_t t = (int64_t)(blockIdx.x & 7) * a.per + (blockIdx.x >> 3);
@@ -289,29 +277,63 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   const int64_t groups = (n + 64 * IT - 1) / (64 * IT);
   const int64_t g0 = groups * strip / a.strips, g1 = groups * (strip + 1) / a.strips;
 
+  // the first rows' loads go out before the queries are read and encoded
+  i32x8 x[KB][IT];
+  int sa[KB][IT];
+  auto load = [&](int64_t n0) {
+          const int last = (int)min((int64_t)(16 * IT), n - n0) - 1;
+          const uint8_t* c0 = a.codes + n0 * (KB * ROWB);
+          const uint8_t* s0 = a.scales + n0 * KB;
+    #pragma unroll
+          for (int i = 0; i < IT; ++i) {
+            const uint32_t row = (uint32_t)min(16 * i + r, last);
+    #pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+              x[kb][i] = row_frag(c0 + (row * KB + kb) * ROWB, g);
+              sa[kb][i] = s0[row * KB + kb];
+            }
+          }
+  };
+  int64_t n0 = (g0 * 4 + w) * 16 * IT;
+  const int64_t end = min(n, g1 * 64 * IT);
+  if (NKB > 0 && n0 < end) load(n0);
+
   const uint8_t* qrow[QT];
   const uint8_t* qsrow[QT];
   i32x8 b[KB][QT];
   int sb[KB][QT];
+  if constexpr (ENC) {
+    // the workgroup encodes its queries once, 16 lanes a block
+    static_assert(QT == 1 && NKB > 0, "at most 16 queries");
+    for (int u = (int)threadIdx.x / LANES; u < a.m * KB; u += 256 / LANES) {
+      const int i = u / KB, kb = u % KB, lane = (int)threadIdx.x % LANES, k = kb * BLK + lane * 8, live = max(0, min(8, a.d - k));
+      float v[8];
+      if (a.q_dtype == TT_F32)
+        ld8n<TT_F32>(a.q, i * a.ldq + k, live, v);
+      else if (a.q_dtype == TT_BF16)
+        ld8n<TT_BF16>(a.q, i * a.ldq + k, live, v);
+      else
+        ld8n<TT_F16>(a.q, i * a.ldq + k, live, v);
+      uint32_t byte;
+      *reinterpret_cast<u32x2*>(enc + u * ROWB + lane * 8) = encode8(v, byte);
+      if (lane == 0) enc[16 * KB * ROWB + u] = (uint8_t)byte;
+    }
+    __syncthreads();
+    const int row = min(r, (int)a.m - 1);
 #pragma unroll
-  for (int j = 0; j < QT; ++j) {
-    const int64_t row = m0 + 16 * j + r, at = min(row, a.m - 1);
-    if constexpr (!ENC) {
+    for (int kb = 0; kb < KB; ++kb) {
+      b[kb][0] = row_frag(enc + (row * KB + kb) * ROWB, g);
+      sb[kb][0] = enc[16 * KB * ROWB + row * KB + kb];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      const int64_t at = min(m0 + 16 * j + r, a.m - 1);
       qrow[j] = (const uint8_t*)a.q + at * nkb * ROWB;
       qsrow[j] = a.qs + at * nkb;
-    }
-    if constexpr (NKB > 0) {
+      if constexpr (NKB > 0) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        if constexpr (ENC) {
-          const int k = kb * BLK + 16 * g;
-          if (a.q_dtype == TT_F32)
-            b[kb][j] = encode_query<TT_F32>(a.q, at * a.ldq, k, a.d, row < a.m, sb[kb][j]);
-          else if (a.q_dtype == TT_BF16)
-            b[kb][j] = encode_query<TT_BF16>(a.q, at * a.ldq, k, a.d, row < a.m, sb[kb][j]);
-          else
-            b[kb][j] = encode_query<TT_F16>(a.q, at * a.ldq, k, a.d, row < a.m, sb[kb][j]);
-        } else {
+        for (int kb = 0; kb < KB; ++kb) {
           b[kb][j] = row_frag(qrow[j] + kb * ROWB, g);
           sb[kb][j] = qsrow[j][kb];
         }
@@ -320,22 +342,6 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   }
 
   if constexpr (NKB > 0) {
-    i32x8 x[KB][IT];
-    int sa[KB][IT];
-    auto load = [&](int64_t n0) {
-      const int last = (int)min((int64_t)(16 * IT), n - n0) - 1;
-      const uint8_t* c0 = a.codes + n0 * (KB * ROWB);
-      const uint8_t* s0 = a.scales + n0 * KB;
-#pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const uint32_t row = (uint32_t)min(16 * i + r, last);
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          x[kb][i] = row_frag(c0 + (row * KB + kb) * ROWB, g);
-          sa[kb][i] = s0[row * KB + kb];
-        }
-      }
-    };
     f32x4 acc[IT][QT];
     auto multiply = [&]() {
 #pragma unroll
@@ -350,11 +356,8 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
           for (int j = 0; j < QT; ++j)
             acc[i][j] = mfma_block<DT>(x[kb][i], b[kb][j], acc[i][j], sa[kb][i], sb[kb][j]);
     };
-    int64_t n0 = (g0 * 4 + w) * 16 * IT;
-    const int64_t end = min(n, g1 * 64 * IT);
     // whole tiles first; addresses of the one after the last stay inside the catalogue
     const int64_t whole = n * Elem<DT>::SIZE * 64 < 0x7FFFFFFF ? end - 16 * IT : -1;
-    if (n0 < end) load(n0);
     while (n0 <= whole) {
       multiply();
       const int64_t at = n0;

@@ -16,6 +16,10 @@ static int ops_launch_check() {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? TT_OK : (int)e;
 }
+// rows in x, CAT_UNIT blocks of them in y
+static dim3 cat_grid(int64_t m, int nkb) {
+  return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>((m + 15) / 16, 16384)), (unsigned)((nkb + CAT_UNIT - 1) / CAT_UNIT));
+}
 static bool dtype_ok(int64_t dt) { return dt == TT_F32 || dt == TT_BF16 || dt == TT_F16; }
 static unsigned grid_for(int64_t work, int64_t per_block, int64_t most) {
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>((work + per_block - 1) / per_block, most));
@@ -81,7 +85,9 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
   a.b1d = hp->beta1;
   a.b2d = hp->beta2;
   a.seed = seed;
-  int64_t chunk = ADAMW_STRIDE;
+  // 8-bit states of many values: 4 rounds a workgroup spare three of four looks for its tensor (96 M values in bf16:
+  // 292 -> 239 us; 32-bit states 517 -> 528 us, small lists want the workgroups)
+  const int64_t chunk = ADAMW_STRIDE * (state_bits == 8 && values >= 1 << 22 ? 4 : 1);
   int64_t last_step = 0;
   AdamwCoef last{};
   for (int32_t from = 0; from < n_tensors;) {
@@ -154,7 +160,7 @@ int32_t tt_cat_write(const void* x, int32_t dtype, int64_t m, int64_t ldx, int32
   }
   if (rows) hipLaunchKernelGGL(k_cat_own, dim3(grid_for(m, 256, 4096)), dim3(256), 0, s, r, m, owner);
   with_dtype(dtype, [&](auto t) {
-    hipLaunchKernelGGL(k_cat_write<decltype(t)::value>, dim3(grid_for(m * nkb, 16, 16384)), dim3(256), 0, s, x, m, ldx,
+    hipLaunchKernelGGL(k_cat_write<decltype(t)::value>, cat_grid(m, nkb), dim3(256), 0, s, x, m, ldx,
                        d, nkb, r, codes, scales, rows ? owner : nullptr);
   });
   if (rows) hipLaunchKernelGGL(k_cat_disown, dim3(grid_for(m, 256, 4096)), dim3(256), 0, s, r, m, owner);
@@ -170,7 +176,7 @@ int32_t tt_cat_read(const uint8_t* codes, const uint8_t* scales, int64_t capacit
   const CatRows r{rows, row0, capacity};
   const int nkb = cat_blocks(d);
   with_dtype(dtype, [&](auto t) {
-    hipLaunchKernelGGL(k_cat_read<decltype(t)::value>, dim3(grid_for(m * nkb, 16, 16384)), dim3(256), 0,
+    hipLaunchKernelGGL(k_cat_read<decltype(t)::value>, cat_grid(m, nkb), dim3(256), 0,
                        (hipStream_t)stream, codes, scales, r, m, d, nkb, out, ldo);
   });
   return ops_launch_check();
@@ -193,7 +199,8 @@ template <int DT, int IT, int QT, int NKB, bool ENC>
 static int launch_stream(StreamArgs& a, hipStream_t s) {
   a.panels = (a.m + 16 * QT - 1) / (16 * QT);
   const int64_t groups = (a.n + 64 * IT - 1) / (64 * IT);
-  const int64_t want = 512 * (QT == 4 ? 1 : 4 / IT);
+  // two workgroups a CU, more where each still has four groups to walk over
+  const int64_t want = QT == 4 ? 512 : std::max<int64_t>(512, std::min<int64_t>(2048, groups / 4));
   a.strips = std::max<int64_t>(1, std::min(groups, (want + a.panels - 1) / a.panels));
   if (a.panels > INT32_MAX / 16 / a.strips) return TT_ERR_UNSUPPORTED;
   a.per = (a.panels * a.strips + 7) / 8;
@@ -254,7 +261,7 @@ int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int3
     uint8_t* qs = qc + m * a.nkb * TT_BLOCK;
     const CatRows r{nullptr, 0, m};
     with_dtype(dtype, [&](auto t) {
-      hipLaunchKernelGGL(k_cat_write<decltype(t)::value>, dim3(grid_for(m * a.nkb, 16, 16384)), dim3(256), 0, s, q, m,
+      hipLaunchKernelGGL(k_cat_write<decltype(t)::value>, cat_grid(m, a.nkb), dim3(256), 0, s, q, m,
                          ldq, d, a.nkb, r, qc, qs, (int32_t*)nullptr);
     });
     a.q = qc;
@@ -269,7 +276,7 @@ int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int3
 
 namespace tt {
 // How dq's rows, columns and sum are split.  Parts of the catalogue until about
-// two workgroups a CU have work, none shorter than 8 steps; a part writes m d
+// two workgroups a CU have work, none shorter than 2 steps; a part writes m d
 // floats and reads its share of the codes and of dS.
 struct DqPlan {
   int ct, rt, wm, groups;
@@ -284,7 +291,7 @@ static DqPlan dq_plan(int64_t m, int64_t n, int32_t d, int32_t dtype) {
   p.mt = (m + 16 * p.rt * p.wm - 1) / (16 * p.rt * p.wm);
   const int64_t step = p.wm == 1 ? 128 : 64, steps = std::max<int64_t>(1, (n + step - 1) / step);
   const int64_t blocks = p.mt * p.groups;
-  int64_t s = std::max<int64_t>(1, std::min<int64_t>((512 + blocks - 1) / blocks, steps / 8));
+  int64_t s = std::max<int64_t>(1, std::min<int64_t>((512 + blocks - 1) / blocks, steps / 2));
   p.part_steps = (steps + s - 1) / s;
   p.splits = (steps + p.part_steps - 1) / p.part_steps;
   return p;
