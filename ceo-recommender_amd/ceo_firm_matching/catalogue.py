@@ -178,7 +178,8 @@ class EmbeddingCatalogue:
             raise ValueError("write: rows or start, not both")
         if m == 0:
             return
-        torch.autograd.graph.increment_version((self.codes, self.scales))  # a backward that saved the old rows must notice
+        if not self.codes.is_inference():  # a backward that saved the old rows must notice
+            torch.autograd.graph.increment_version((self.codes, self.scales))
         if self.device.type != "cuda":
             codes, scales = block8.encode(emb)
             if rows is None:

@@ -113,6 +113,13 @@ class AdamW(torch.optim.Optimizer):
         if not g["weight_decay"] >= 0 or not np.isfinite(g["weight_decay"]):
             raise ValueError(f"Invalid weight_decay value: {g['weight_decay']}")
 
+    @staticmethod
+    def _check_apart(params):
+        """One launch updates all of them: no value may be in two."""
+        at = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(at, at[1:])):
+            raise ValueError("AdamW: parameters of a group share memory (the same parameter twice, or overlapping views)")
+
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
         g = self.param_groups[-1]
@@ -127,6 +134,7 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("AdamW: one device per parameter group")
                 if p.device.type not in ("cuda", "cpu"):
                     raise NotImplementedError(f"AdamW: HIP or CPU parameters, got {p.device}")
+            self._check_apart(g["params"])
             if self._capturable and g["params"] and g["params"][0].device.type != "cuda":
                 raise ValueError("AdamW: capturable needs parameters on a HIP device")
         except Exception:
@@ -183,15 +191,13 @@ class AdamW(torch.optim.Optimizer):
             t[:, 1] = [x.data_ptr() for x in grads]
             if self._capturable:
                 t[:, 4] = range(len(params)) if live is None else live
-            elif live is None:
-                b.host_steps += 1
-                t[:, 4] = b.host_steps
             else:
-                b.host_steps[live] += 1
-                t[:, 4] = b.host_steps[live]
+                t[:, 4] = (b.host_steps if live is None else b.host_steps[live]) + 1
             hp = N.TTAdamWHP(g["lr"], g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"])
             N.check(N.lib().tt_adamw_step(at or t.ctypes.data, len(params), self._bits, ctypes.byref(b.native),
                                           ctypes.byref(hp), self._seed, N.stream_ptr(b.device)), "tt_adamw_step")
+            if not self._capturable:  # the step was taken
+                b.host_steps[slice(None) if live is None else live] = t[:, 4]
         torch.autograd.graph.increment_version(params)
 
     def _step_cpu(self, g, b, live, grads):

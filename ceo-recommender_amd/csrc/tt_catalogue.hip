@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) void k_cat_read(const uint8_t* codes, const ui
 // stay in the accumulator.  The 8-bit matrix instructions cut the products of
 // one instruction off below the largest of them (measured over all e4m3
 // values: a sum of 128 is off by up to 2^-11 of its largest product, 5e-5 of
-// the result in the 2-norm), far below the results' own rounding (2^-9, 2^-12)
+// the result in the 2-norm), far below the results' own rounding (2^-8, 2^-11)
 // but not a sum in 32 bits.
 // Results in 32 bits: both operands decoded to bf16, exactly, and
 // v_mfma_f32_16x16x32_bf16, whose sums measured 8e-8.

@@ -4,7 +4,6 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
-#include <mutex>
 #include <type_traits>
 
 #include "tt_adamw.hip"
@@ -21,6 +20,8 @@ static dim3 cat_grid(int64_t m, int nkb) {
   return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>((m + 15) / 16, 16384)), (unsigned)((nkb + CAT_UNIT - 1) / CAT_UNIT));
 }
 static bool dtype_ok(int64_t dt) { return dt == TT_F32 || dt == TT_BF16 || dt == TT_F16; }
+static bool aligned(const void* p, uintptr_t to) { return (uintptr_t)p % to == 0; }
+static uintptr_t size_of(int32_t dt) { return dt == TT_F32 ? 4 : 2; }
 static unsigned grid_for(int64_t work, int64_t per_block, int64_t most) {
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>((work + per_block - 1) / per_block, most));
 }
@@ -55,8 +56,8 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
     const tt_adamw_tensor& t = tensors[i];
     if (t.n < 0 || !dtype_ok(t.dtype)) return TT_ERR_ARG;
     if (t.n == 0) continue;
-    const int64_t align = t.dtype == TT_F32 ? 4 : 2;
-    if (!t.param || !t.grad || (uintptr_t)t.param % align || (uintptr_t)t.grad % align) return TT_ERR_ARG;
+    const uintptr_t es = size_of((int32_t)t.dtype);
+    if (!t.param || !t.grad || !aligned(t.param, es) || !aligned(t.grad, es)) return TT_ERR_ARG;
     const int64_t nb = (t.n - 1) / TT_BLOCK + 1;
     if (t.block0 < 0 || nb > state->n_blocks || t.block0 > state->n_blocks - nb) return TT_ERR_ARG;
     if (state->steps ? t.step < 0 || t.step >= state->n_steps : t.step < 1) return TT_ERR_ARG;
@@ -65,6 +66,8 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
   if (values == 0) return TT_OK;
   if (state_bits == 32 ? !state->exp_avg || !state->exp_avg_sq
                        : !state->m_codes || !state->m_scales || !state->r_codes || !state->r_scales)
+    return TT_ERR_ARG;
+  if (!aligned(state->exp_avg, 4) || !aligned(state->exp_avg_sq, 4) || !aligned(state->steps, 8) || !aligned(state->coefs, 4))
     return TT_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   AdamwArgs a;
@@ -131,6 +134,7 @@ int32_t tt_adamw_held(const tt_adamw_state* state, void* m, void* r, tt_stream_t
   if (!state || state->n_blocks < 0) return TT_ERR_ARG;
   if (state->n_blocks == 0) return TT_OK;
   if (!state->m_codes || !state->m_scales || !state->r_codes || !state->r_scales || !m || !r) return TT_ERR_ARG;
+  if (!aligned(m, 2) || !aligned(r, 2)) return TT_ERR_ARG;
   const int64_t n8 = state->n_blocks * b8::LANES;
   hipLaunchKernelGGL(k_adamw_held, dim3(grid_for(n8, 256, 8192), 2), dim3(256), 0, (hipStream_t)stream, state->m_codes,
                      state->m_scales, state->r_codes, state->r_scales, m, r, n8);
@@ -147,7 +151,7 @@ int32_t tt_cat_write(const void* x, int32_t dtype, int64_t m, int64_t ldx, int32
   if (rows && (m >= INT32_MAX || (m > 0 && !owner))) return TT_ERR_ARG;  // a row's owner is a place in 31 bits
   if (!rows && (row0 < 0 || row0 > capacity - m)) return TT_ERR_ARG;
   if (m == 0 || capacity == 0) return TT_OK;
-  if (!x || !codes || !scales) return TT_ERR_ARG;
+  if (!x || !codes || !scales || !aligned(x, size_of(dtype)) || !aligned(rows, 8) || !aligned(owner, 4)) return TT_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   const CatRows r{rows, row0, capacity};
   const int nkb = cat_blocks(d);
@@ -172,7 +176,7 @@ int32_t tt_cat_read(const uint8_t* codes, const uint8_t* scales, int64_t capacit
   if (!cat_sizes_ok(m, d) || !cat_sizes_ok(capacity, d) || !dtype_ok(dtype) || (m > 1 && ldo < d)) return TT_ERR_ARG;
   if (!rows && (row0 < 0 || row0 > capacity - m)) return TT_ERR_ARG;
   if (m == 0) return TT_OK;
-  if (!out || (capacity > 0 && (!codes || !scales))) return TT_ERR_ARG;
+  if (!out || (capacity > 0 && (!codes || !scales)) || !aligned(out, size_of(dtype)) || !aligned(rows, 8)) return TT_ERR_ARG;
   const CatRows r{rows, row0, capacity};
   const int nkb = cat_blocks(d);
   with_dtype(dtype, [&](auto t) {
@@ -243,6 +247,7 @@ int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int3
   if (m == 0 || n == 0) return TT_OK;
   const int64_t need = tt_cat_scores_workspace_bytes(m, n, d);
   if (!q || !codes || !scales || !out || (need > 0 && !ws)) return TT_ERR_ARG;
+  if (!aligned(q, size_of(dtype)) || !aligned(out, size_of(out_dtype)) || !aligned(codes, 16) || !aligned(ws, 16)) return TT_ERR_ARG;
   if (ws_bytes < need) return TT_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   StreamArgs a{};
@@ -300,10 +305,8 @@ static DqPlan dq_plan(int64_t m, int64_t n, int32_t d, int32_t dtype) {
 template <int DT, int DQ, int CT, int RT, int WM, bool ODD>
 static void launch_dq_as(const DqArgs& a, hipStream_t s) {
   constexpr int LDS = dq_lds<CT, WM>();
-  static std::once_flag once;
-  std::call_once(once, [] {
+  if constexpr (LDS > 64 * 1024)  // (every time: it holds for the current device)
     (void)hipFuncSetAttribute((const void*)k_cat_dq<DT, DQ, CT, RT, WM, ODD>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-  });
   hipLaunchKernelGGL((k_cat_dq<DT, DQ, CT, RT, WM, ODD>), dim3((unsigned)(8 * a.per)), dim3(256), LDS, s, a);
 }
 template <int DT, int DQ, int CT, int RT, int WM>
@@ -351,6 +354,7 @@ int32_t tt_cat_dq(const void* ds, int32_t ds_dtype, int64_t m, int64_t lds, int6
   if (!dq || (n > 0 && (!ds || !codes || !scales))) return TT_ERR_ARG;
   const int64_t need = tt_cat_dq_workspace_bytes(m, n, d, ds_dtype);
   if (need > 0 && (!ws || ws_bytes < need)) return TT_ERR_WORKSPACE;
+  if (!aligned(ds, size_of(ds_dtype)) || !aligned(dq, size_of(dq_dtype)) || !aligned(codes, 16) || !aligned(ws, 16)) return TT_ERR_ARG;
   const DqPlan p = dq_plan(m, n, d, ds_dtype);
   if (p.mt > INT32_MAX / 16 / p.groups / p.splits) return TT_ERR_UNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;

@@ -529,7 +529,9 @@ int32_t tt_adamw_held(const tt_adamw_state* state, void* m, void* r, tt_stream_t
  * rows[i] (device int64), or row0 + i when rows == NULL; rows outside
  * [0, capacity) are left out of a write and read as zeros.  A row named twice
  * in one write takes the values of its last mention; owner [capacity] (device
- * int32, zero before the first call and after each) is needed with rows.    */
+ * int32, zero before the first call and after each) is needed with rows.
+ * codes and ws lie on 16-byte boundaries for scores and gradient, every other
+ * pointer on its type's.                                                    */
 int32_t tt_cat_write(const void* x, int32_t dtype, int64_t m, int64_t ldx, int32_t d,
                      const int64_t* rows, int64_t row0, uint8_t* codes, uint8_t* scales,
                      int64_t capacity, int32_t* owner, tt_stream_t stream);

@@ -202,6 +202,10 @@ def test_refusals():
         AdamW([torch.nn.Parameter(torch.ones(4, dtype=torch.float64))])
     with pytest.raises(ValueError):
         AdamW([torch.nn.Parameter(torch.ones(4, 3).t())])
+    both = torch.zeros(10)
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([torch.nn.Parameter(both[:6]), torch.nn.Parameter(both[5:])])
+    AdamW([torch.nn.Parameter(both[:5]), torch.nn.Parameter(both[5:])])
     opt = AdamW([p], state_bits=8)
     with pytest.raises(ValueError):
         opt.load_state_dict(AdamW([p]).state_dict())  # 32-bit states into 8-bit ones
@@ -241,7 +245,8 @@ def test_host_argument_errors():
                dict(state=N.TTAdamWState(n_blocks=4)), dict(bits=8, state=N.TTAdamWState(exp_avg=at, exp_avg_sq=at, n_blocks=4)),
                dict(state=N.TTAdamWState(exp_avg=at, exp_avg_sq=at, n_blocks=4, steps=at)),
                dict(state=N.TTAdamWState(exp_avg=at, exp_avg_sq=at, n_blocks=4, steps=at, coefs=at, n_steps=1)),
-               dict(block0=2 ** 62), dict(n=2 ** 62)):
+               dict(block0=2 ** 62), dict(n=2 ** 62), dict(grad=at + 1, dtype=N.TT_BF16),
+               dict(state=N.TTAdamWState(exp_avg=at + 2, exp_avg_sq=at, n_blocks=4))):
         assert call(**kw) == N.TT_ERR_ARG, kw
     assert L.tt_adamw_held(None, at, at, None) == N.TT_ERR_ARG
     assert L.tt_adamw_held(ctypes.byref(st), None, at, None) == N.TT_ERR_ARG

@@ -174,7 +174,7 @@ def test_host_argument_errors():
 
     assert write(m=0) == N.TT_OK
     for kw in (dict(x=None), dict(dt=3), dict(m=-1), dict(ldx=7), dict(d=0), dict(d=1 << 21), dict(row0=3), dict(row0=-1),
-               dict(codes=None), dict(scales=None), dict(cap=-1), dict(rows=p, owner=None), dict(rows=p, m=2 ** 31),
+               dict(codes=None), dict(scales=None), dict(cap=-1), dict(rows=p, owner=None), dict(rows=p, m=2 ** 31), dict(x=p + 2), dict(rows=p + 4),
                dict(m=2 ** 41, cap=2 ** 41)):
         assert write(**kw) == N.TT_ERR_ARG, kw
 
@@ -190,17 +190,28 @@ def test_host_argument_errors():
 
     assert scores(m=0) == N.TT_OK and scores(n=0) == N.TT_OK
     for kw in (dict(q=None), dict(dt=5), dict(odt=5), dict(ldq=7), dict(codes=None), dict(scales=None), dict(out=None),
-               dict(d=0), dict(m=-2), dict(n=-1)):
+               dict(d=0), dict(m=-2), dict(n=-1), dict(q=p + 1, dt=1), dict(out=p + 2), dict(codes=p + 8)):
         assert scores(**kw) == N.TT_ERR_ARG, kw
     assert L.tt_cat_scores_workspace_bytes(-1, 4, 8) == N.TT_ERR_ARG
+    need = L.tt_cat_scores_workspace_bytes(20, 4, 8)
+    assert need > 0 and scores(m=20, wsb=need - 1) == N.TT_ERR_WORKSPACE and scores(m=20, ws=None, wsb=need) == N.TT_ERR_ARG
+    assert scores(m=20, ws=p + 8, wsb=need) == N.TT_ERR_ARG
     assert L.tt_cat_dq_workspace_bytes(4, 4, 0, 0) == N.TT_ERR_ARG
 
     def dq(ds=p, dt=0, m=2, lds=4, n=4, codes=p, scales=p, d=8, out=p, odt=0, ws=p, wsb=1 << 30):
         return L.tt_cat_dq(ds, dt, m, lds, n, codes, scales, d, out, odt, ws, wsb, None)
 
     assert dq(m=0) == N.TT_OK
-    for kw in (dict(ds=None), dict(dt=7), dict(odt=7), dict(lds=3), dict(codes=None), dict(out=None), dict(d=0), dict(n=-1)):
+    for kw in (dict(ds=None), dict(dt=7), dict(odt=7), dict(lds=3), dict(codes=None), dict(out=None), dict(d=0), dict(n=-1),
+               dict(codes=p + 8), dict(ds=p + 2), dict(out=p + 1, odt=1)):
         assert dq(**kw) == N.TT_ERR_ARG, kw
+
+
+def test_inference_mode():
+    with torch.inference_mode():
+        cat = EmbeddingCatalogue(3, 5)
+        cat.write(torch.ones(3, 5))
+        assert torch.equal(cat.scores(torch.ones(2, 5)), torch.full((2, 3), 5.0))
 
 
 def test_block_scale_is_the_smallest_that_fits():

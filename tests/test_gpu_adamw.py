@@ -242,3 +242,33 @@ def test_long_run_tracks_the_second_moment(dev):
     m32, v32 = (x.reshape(-1)[:10000] for x in o32.held_states())
     assert abs(float(r8.square().mean() / v32.mean()) - 1) < 0.05
     assert abs(float((m8 * m32).mean() / m32.square().mean()) - 1) < 0.05
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_2_31_values(dev, bits):
+    n = 2 ** 31 + 1000
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device=dev))
+    opt = AdamW([p], lr=1e-2, state_bits=bits, weight_decay=0.0)
+    g = torch.zeros(n, dtype=torch.bfloat16, device=dev)
+    places = [0, 2 ** 31 - 1, 2 ** 31, n - 1]
+    for at in places:
+        g[at] = 1.0
+    p.grad = g
+    opt.step()
+    assert sum(int(part.count_nonzero()) for part in p.detach().split(1 << 28)) == 4
+    # the first step moves by lr whatever the gradient's size
+    assert [float(p.detach()[at]) for at in places] == [float(torch.tensor(-1e-2).bfloat16())] * 4
+
+
+def test_a_refused_step_changes_nothing(dev):
+    (p,) = make([(50,)], [torch.float32], dev)
+    opt = AdamW([p])
+    p.grad = torch.ones(50, device=dev)
+    before = p.detach().clone()
+    opt.param_groups[0]["lr"] = float("nan")
+    with pytest.raises(ValueError):
+        opt.step()
+    assert torch.equal(p.detach(), before) and int(opt.state[p]["step"]) == 0
+    opt.param_groups[0]["lr"] = 1e-3
+    opt.step()
+    assert int(opt.state[p]["step"]) == 1 and not torch.equal(p.detach(), before)

@@ -341,3 +341,50 @@ def test_training_against_the_catalogue_and_adamw(dev):
         assert rel < 10 * 2.0 ** -4, rel
         opt.step()
     assert all(torch.isfinite(p).all() for p in net.parameters())
+
+
+def test_offsets_past_32_bits(dev):
+    """A catalogue of more than 2^32 bytes; scores and upstream gradients of
+    more than 2^32 bytes: values at both ends."""
+    n, d = 17_000_003, 256
+    cat = EmbeddingCatalogue(n, d, device=dev)
+    x = torch.nn.functional.normalize(torch.randn(200, d, device=dev), dim=1)
+    cat.write(x[:100])
+    cat.write(x[100:], start=n - 100)
+    assert torch.equal(cat.read(start=n - 100), cat.read(rows=torch.arange(n - 100, n, device=dev)))
+    small = EmbeddingCatalogue(200, d, device=dev)
+    small.write(x)
+    assert torch.equal(cat.read(start=n - 100), small.read(start=100))
+    q = torch.nn.functional.normalize(torch.randn(130, d, device=dev), dim=1).bfloat16()
+    want = small.scores(q)
+    for m in (1, 20, 130):  # 130 x n in bf16 is 4.4e9 bytes
+        qm = q[:m].clone().requires_grad_()
+        s = cat.scores(qm)
+        # few and many queries sum in other orders: each is within its own bound of the exact score
+        for part, ref in ((s[:, :100], want[:m, :100]), (s[:, n - 100:], want[:m, 100:])):
+            assert float((part.detach().float() - ref.float()).abs().max()) <= 2 * (2.0 ** -8 + 2.0 ** -10)  # |scores| <= 1: half a step of bf16
+        assert not s[:, 100:n - 100:100003].any()
+        ds = torch.zeros(m, n, dtype=torch.bfloat16, device=dev)
+        ds[:, :100], ds[:, n - 100:] = 0.5, -0.25
+        g = torch.autograd.grad(s, qm, ds)[0]
+        v = small.read().double()
+        row = 0.5 * v[:100].sum(0) - 0.25 * v[100:].sum(0)
+        tol = 2.0 ** -8 * row.abs() * 1.01 + (200 + 64) * 2.0 ** -23 * v.abs().sum(0)
+        assert bool(((g.double() - row).abs() <= tol).all())
+        del s, ds, g
+
+
+@pytest.mark.parametrize("n", [64, 65, 127, 128, 129, 191, 193, 257, 511, 513])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_of_odd_length_read_no_neighbour(dev, n, dtype):
+    """The gradient of 16-bit rows at odd distances, next to NaN in front of,
+    between and behind the rows."""
+    for m in (2, 33, 130):
+        cat, q, ds = score_case(dev, m, n, 96, dtype, dtype, n)
+        want = torch.autograd.grad(cat.scores(q), q, ds.to(dev))[0]
+        for before, gap in ((0, 0), (0, 2), (2, 2), (1, 1), (1, 2), (4, 3)):
+            store = torch.full((before + m * (n + gap) + 2,), float("nan"), dtype=dtype, device=dev)
+            view = store[before:before + m * (n + gap)].view(m, n + gap)[:, :n]
+            view.copy_(ds)
+            got = torch.autograd.grad(cat.scores(q), q, view)[0]
+            assert torch.equal(got, want), (m, before, gap)
