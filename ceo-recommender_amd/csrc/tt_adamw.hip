@@ -5,7 +5,13 @@
 //
 // k_adamw takes up to ADAMW_LIST tensors by value (kernel arguments, so a
 // captured graph keeps them): a workgroup finds its tensor from the prefix of
-// chunk counts, then walks its chunk 8 consecutive values a thread.
+// chunk counts, one lane a tensor, then walks its chunk.
+//
+// 32-bit states are bound by memory (28 bytes a value in fp32): 96 M values
+// 499 us, 5.4 TB/s.  8-bit states in bf16 (10 bytes a value) by instructions, about
+// 60 a value of which the rounding hash takes 15: 96 M values 236 us; reading the
+// values back (k_adamw_held) 92 us, 6.3 TB/s.  The 21 tensors of the two
+// towers take 3.7 and 4.6 us, launch and latency.
 #include "tt_block8.h"
 
 namespace tt {

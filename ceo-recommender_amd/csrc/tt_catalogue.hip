@@ -23,7 +23,9 @@ __global__ __launch_bounds__(256) void k_cat_own(CatRows r, int64_t m, int32_t* 
 }
 
 // 16 lanes take up to CAT_UNIT blocks of a row (blockIdx.y: which ones), 8
-// values each: all loads first, one row number and one owner for all of them
+// values each: all loads first, one row number and one owner for all of them.
+// Bound by memory: a million rows of 256 in bf16 written 152 us (5.1 TB/s),
+// read 124 us (6.3 TB/s); a division a block instead of blockIdx.y 158, 135 us
 constexpr int CAT_UNIT = 2;
 template <int DT>
 __global__ __launch_bounds__(256) void k_cat_write(const void* x, int64_t m, int64_t ldx, int d, int nkb, CatRows r,
@@ -173,18 +175,8 @@ __device__ __forceinline__ i32x8 lds_frag(const uint8_t* s, int row, int g) {
   return frag_of(*reinterpret_cast<const u32x4*>(s + lds_chunk(row, g)),
                  *reinterpret_cast<const u32x4*>(s + lds_chunk(row, g + 4)));
 }
-// 16 bytes a lane from global memory straight into LDS at base + 16 lane
-__device__ __forceinline__ void ld_lds16(const uint8_t* g, uint8_t* s) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                   (__attribute__((address_space(3))) void*)s, 16, 0, 0);
-}
+// loads straight into LDS have arrived
 __device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-// a barrier that orders LDS alone: loads and stores of global memory stay in flight
-__device__ __forceinline__ void block_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
 
 template <int DT>
 __device__ __forceinline__ f32x4 mfma_block(const i32x8& a, const i32x8& b, const f32x4& c, int sa, int sb) {
@@ -244,11 +236,14 @@ __device__ __forceinline__ void store_tile(uint8_t* so, const f32x4 (&acc)[IT][Q
   __builtin_amdgcn_wave_barrier();
 }
 
-// Few blocks a row (or few queries): a wave keeps 16 QT queries in registers
-// and walks over the catalogue, 16 IT rows at a time, straight from global
-// memory: no barrier, and the next rows' loads fly while this tile is stored.
-// The 4 waves of a workgroup take neighbouring row groups, so that a query's
-// results go out in pieces of 64 IT values.
+// Up to 64 queries, bound by the catalogue's bytes: a wave keeps 16 QT queries
+// in registers and walks over the catalogue, 16 IT rows at a time, straight
+// from global memory: no barrier, and the next rows' loads fly while this tile
+// is stored.  The 4 waves of a workgroup take neighbouring row groups, so that
+// a query's results go out in pieces of 64 IT values.  Measured: 1 x 1000003 x
+// 128 21.6 us (6.1 TB/s), 16 x 1000003 x 128 27 us (6.0 TB/s), 1 x 100000 x 256
+// 8.2 us.  For more queries the tiles below are faster (8192 x 100000 x 256: 776
+// against 420 us: every wave reads the catalogue through L2 again).
 struct StreamArgs {
   const void* q;            // raw queries (ENC) or their codes
   const uint8_t* qs;        // their scale bytes (not ENC)
@@ -281,18 +276,18 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   i32x8 x[KB][IT];
   int sa[KB][IT];
   auto load = [&](int64_t n0) {
-          const int last = (int)min((int64_t)(16 * IT), n - n0) - 1;
-          const uint8_t* c0 = a.codes + n0 * (KB * ROWB);
-          const uint8_t* s0 = a.scales + n0 * KB;
-    #pragma unroll
-          for (int i = 0; i < IT; ++i) {
-            const uint32_t row = (uint32_t)min(16 * i + r, last);
-    #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-              x[kb][i] = row_frag(c0 + (row * KB + kb) * ROWB, g);
-              sa[kb][i] = s0[row * KB + kb];
-            }
-          }
+    const int last = (int)min((int64_t)(16 * IT), n - n0) - 1;
+    const uint8_t* c0 = a.codes + n0 * (KB * ROWB);
+    const uint8_t* s0 = a.scales + n0 * KB;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const uint32_t row = (uint32_t)min(16 * i + r, last);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        x[kb][i] = row_frag(c0 + (row * KB + kb) * ROWB, g);
+        sa[kb][i] = s0[row * KB + kb];
+      }
+    }
   };
   int64_t n0 = (g0 * 4 + w) * 16 * IT;
   const int64_t end = min(n, g1 * 64 * IT);
@@ -639,6 +634,10 @@ __device__ __forceinline__ void ds_planes(const DsFrag<DT>& f, bf16x8 (&a)[PL]) 
   }
 }
 
+// Bound by dS's bytes up to 128 columns, then by what LDS hands the waves.
+// Measured in bf16: 16384 x 32768 x 128 242 us (4.5 TB/s), x 32771 330 us, 8192 x
+// 100000 x 256 551 us (3.0 TB/s).  16 rows a wave (RT = 1) read LDS twice as often:
+// 826 against 701 us at 8192 x 131072 x 256.
 // One workgroup: 16 RT WM rows of dS against a part of the catalogue, 16 CT
 // columns of dq in its waves' accumulators.  A step of DQ_STEP catalogue rows
 // is decoded once into LDS as bf16 [row][column] and read back transposed; the

@@ -260,12 +260,12 @@ def test_repeatable(dev):
         assert all(torch.equal(a, runs[0][0]) and torch.equal(b, runs[0][1]) for a, b in runs)
 
 
-@pytest.mark.parametrize("m", [1, 24, 300])
-def test_captured_together(dev, m):
+@pytest.mark.parametrize("m,d", [(1, 100), (24, 100), (300, 100), (20, 200), (300, 300)])
+def test_captured_together(dev, m, d):
     """A training step against the catalogue in one graph -- indexed write,
     scores, softmax loss, gradient -- replayed with eager work between; two
     graphs of the same catalogue alternate."""
-    d, n = 100, 700
+    n = 700
     cat, q, _ = score_case(dev, m, n, d, torch.float32, torch.float32)
     new = torch.randn(30, d, device=dev)
     rows = torch.randint(0, n, (30,), device=dev)
