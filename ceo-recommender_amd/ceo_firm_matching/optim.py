@@ -28,8 +28,8 @@ class _Bucket:
     def __init__(self, params, bits, capturable):
         self.params = params
         self.device = params[0].device if params else torch.device("cpu")
-        self.index = -1 if self.device.type == "cpu" else self.device.index  # Tensor.get_device()
         self.numel = [p.numel() for p in params]
+        self.like = [(p.numel(), p.dtype, p.get_device()) for p in params]  # what a step has to find
         nb = [block8.blocks_of(n) for n in self.numel]
         self.block0 = [0] * len(nb)
         for i in range(1, len(nb)):
@@ -167,10 +167,11 @@ class AdamW(torch.optim.Optimizer):
                 dense = [False]
             if not params:
                 continue
-            sizes = b.numel if live is None else [b.numel[i] for i in live]
-            if ([p.numel() for p in params] != sizes or {p.get_device() for p in params} != {b.index}
-                    or not all([p.is_contiguous() for p in params])):
-                raise RuntimeError("AdamW: a parameter changed its size, device or layout after the optimizer was made")
+            like = b.like if live is None else [b.like[i] for i in live]
+            if [(p.numel(), p.dtype, p.get_device()) for p in params] != like or not all([p.is_contiguous() for p in params]):
+                raise RuntimeError("AdamW: a parameter changed its size, type, device or layout after the optimizer was made")
+            if [(x.numel(), x.dtype, x.get_device()) for x in grads] != like:
+                raise RuntimeError("AdamW: a gradient's size, type or device is not its parameter's")
             if not all(dense):
                 if any(x.layout != torch.strided for x in grads):
                     raise NotImplementedError("AdamW: sparse gradients are not supported")

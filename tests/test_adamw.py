@@ -217,10 +217,19 @@ def test_refusals():
     with pytest.raises(NotImplementedError):
         o.step()
     p.grad = torch.ones(4)
-    p.data = torch.ones(9)
-    p.grad = torch.ones(9)
-    with pytest.raises(RuntimeError):
-        opt.step()
+    for other in (torch.ones(9), torch.ones(4, dtype=torch.bfloat16), torch.ones(8)[::2]):
+        q = torch.nn.Parameter(torch.ones(4))
+        o = AdamW([q], state_bits=8)
+        q.data = other
+        q.grad = torch.ones_like(other)
+        with pytest.raises(RuntimeError, match="parameter changed"):
+            o.step()
+    q = torch.nn.Parameter(torch.ones(9))
+    q.grad = torch.ones(9)
+    q.data = torch.ones(4)  # the gradient is of the old size
+    o = AdamW([q])
+    with pytest.raises(RuntimeError, match="gradient"):
+        o.step()
 
 
 def test_host_argument_errors():
