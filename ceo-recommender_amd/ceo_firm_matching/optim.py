@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 from itertools import chain
+from operator import attrgetter
 from typing import Optional
 
 import numpy as np
@@ -17,6 +18,15 @@ import torch
 
 from . import _native as N
 from . import block8
+
+# over lists of parameters at every step: called without a Python frame each
+_grad, _dtype = attrgetter("grad"), attrgetter("dtype")
+_numel, _contiguous, _address = torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+
+
+def _likeness(tensors):
+    return [list(map(_numel, tensors)), list(map(_dtype, tensors)), list(map(torch.Tensor.get_device, tensors))]
+
 
 _BYTES = ("exp_avg_codes", "exp_avg_scales", "exp_avg_sqrt_codes", "exp_avg_sqrt_scales")
 
@@ -29,7 +39,7 @@ class _Bucket:
         self.params = params
         self.device = params[0].device if params else torch.device("cpu")
         self.numel = [p.numel() for p in params]
-        self.like = [(p.numel(), p.dtype, p.get_device()) for p in params]  # what a step has to find
+        self.like = _likeness(params)  # what a step has to find
         nb = [block8.blocks_of(n) for n in self.numel]
         self.block0 = [0] * len(nb)
         for i in range(1, len(nb)):
@@ -156,10 +166,10 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for g, b in zip(self.param_groups, self._buckets):
-            live, params, grads = None, b.params, [p.grad for p in b.params]
+            live, params, grads = None, b.params, list(map(_grad, b.params))
             try:
-                dense = [x.is_contiguous() for x in grads]
-            except AttributeError:  # parameters without a gradient among them
+                dense = list(map(_contiguous, grads))
+            except TypeError:  # parameters without a gradient among them
                 live = [i for i, x in enumerate(grads) if x is not None]
                 params, grads = [params[i] for i in live], [grads[i] for i in live]
                 dense = [x.layout == torch.strided and x.is_contiguous() for x in grads]
@@ -167,10 +177,10 @@ class AdamW(torch.optim.Optimizer):
                 dense = [False]
             if not params:
                 continue
-            like = b.like if live is None else [b.like[i] for i in live]
-            if [(p.numel(), p.dtype, p.get_device()) for p in params] != like or not all([p.is_contiguous() for p in params]):
+            like = b.like if live is None else [[x[i] for i in live] for x in b.like]
+            if _likeness(params) != like or not all(map(_contiguous, params)):
                 raise RuntimeError("AdamW: a parameter changed its size, type, device or layout after the optimizer was made")
-            if [(x.numel(), x.dtype, x.get_device()) for x in grads] != like:
+            if _likeness(grads) != like:
                 raise RuntimeError("AdamW: a gradient's size, type or device is not its parameter's")
             if not all(dense):
                 if any(x.layout != torch.strided for x in grads):
@@ -188,8 +198,8 @@ class AdamW(torch.optim.Optimizer):
             if not self._capturable and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: a captured step needs capturable=True (the step count would be frozen)")
             t, at = (b.table, b.table_at) if live is None else (b.table[live], 0)
-            t[:, 0] = [p.data_ptr() for p in params]
-            t[:, 1] = [x.data_ptr() for x in grads]
+            t[:, 0] = list(map(_address, params))
+            t[:, 1] = list(map(_address, grads))
             if self._capturable:
                 t[:, 4] = range(len(params)) if live is None else live
             else:
