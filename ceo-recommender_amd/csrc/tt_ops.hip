@@ -148,9 +148,10 @@ static int cat_blocks(int32_t d) { return (d + TT_BLOCK - 1) / TT_BLOCK; }
 int32_t tt_cat_write(const void* x, int32_t dtype, int64_t m, int64_t ldx, int32_t d, const int64_t* rows, int64_t row0,
                      uint8_t* codes, uint8_t* scales, int64_t capacity, int32_t* owner, tt_stream_t stream) {
   if (!cat_sizes_ok(m, d) || !cat_sizes_ok(capacity, d) || !dtype_ok(dtype) || (m > 1 && ldx < d)) return TT_ERR_ARG;
-  if (rows && (m >= INT32_MAX || (m > 0 && !owner))) return TT_ERR_ARG;  // a row's owner is a place in 31 bits
+  if (rows && m >= INT32_MAX) return TT_ERR_ARG;  // a row's owner is a place in 31 bits
   if (!rows && (row0 < 0 || row0 > capacity - m)) return TT_ERR_ARG;
   if (m == 0 || capacity == 0) return TT_OK;
+  if (rows && !owner) return TT_ERR_ARG;
   if (!x || !codes || !scales || !aligned(x, size_of(dtype)) || !aligned(rows, 8) || !aligned(owner, 4)) return TT_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   const CatRows r{rows, row0, capacity};

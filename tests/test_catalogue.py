@@ -133,7 +133,9 @@ def test_shapes_views_and_empty_calls():
     cat.write(x[:0])
     cat.write(x[:0], rows=torch.zeros(0, dtype=torch.int64))
     assert cat.read(count=0).shape == (0, 33)
-    assert EmbeddingCatalogue(0, 5).scores(torch.zeros(2, 5)).shape == (2, 0)
+    empty = EmbeddingCatalogue(0, 5)
+    empty.write(torch.zeros(2, 5), rows=torch.tensor([0, -1]))
+    assert empty.scores(torch.zeros(2, 5)).shape == (2, 0) and not empty.read(rows=torch.tensor([0])).any()
     other = EmbeddingCatalogue.from_storage(cat.codes, cat.scales, 33)
     assert torch.equal(other.read(), cat.read())
     s = cat.scores(x.clone().requires_grad_())

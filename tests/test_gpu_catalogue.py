@@ -388,3 +388,21 @@ def test_rows_of_odd_length_read_no_neighbour(dev, n, dtype):
             view.copy_(ds)
             got = torch.autograd.grad(cat.scores(q), q, view)[0]
             assert torch.equal(got, want), (m, before, gap)
+
+
+def test_empty_calls(dev):
+    empty = EmbeddingCatalogue(0, 5, device=dev)
+    empty.write(torch.zeros(2, 5, device=dev), rows=torch.tensor([0, -1], device=dev))
+    q = torch.ones(2, 5, device=dev, requires_grad=True)
+    s = empty.scores(q)
+    assert s.shape == (2, 0) and not empty.read(rows=torch.tensor([0], device=dev)).any()
+    s.sum().backward()
+    assert not q.grad.any()
+    cat = EmbeddingCatalogue(7, 5, device=dev)
+    none = torch.zeros(0, 5, device=dev, requires_grad=True)
+    cat.write(none)
+    cat.write(none, rows=torch.zeros(0, dtype=torch.int64, device=dev))
+    s = cat.scores(none)
+    assert s.shape == (0, 7) and cat.read(rows=torch.zeros(0, dtype=torch.int64, device=dev)).shape == (0, 5)
+    s.sum().backward()
+    assert none.grad.shape == (0, 5)
