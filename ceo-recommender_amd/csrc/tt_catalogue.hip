@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   using namespace b8;
   constexpr int KB = NKB ? NKB : 1;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * tile_lds<DT, IT, QT>()];
-  __shared__ __attribute__((aligned(16))) uint8_t enc[ENC ? 16 * KB * (ROWB + 1) : 16];  // ENC: the queries' codes, scale bytes
+  __shared__ __attribute__((aligned(16))) uint8_t enc[ENC ? 16 * QT * KB * (ROWB + 1) : 16];  // ENC: the queries' codes, scale bytes
   const int l = lane_id(), w = wave_id(), r = l & 15, g = l >> 4;
   uint8_t* const so = lds + w * tile_lds<DT, IT, QT>();
   const int64_t t = (int64_t)(blockIdx.x & 7) * a.per + (blockIdx.x >> 3);
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   int sb[KB][QT];
   if constexpr (ENC) {
     // the workgroup encodes its queries once, 16 lanes a block
-    static_assert(QT == 1 && NKB > 0, "at most 16 queries");
+    static_assert(NKB > 0, "the codes stay in registers");
     for (int u = (int)threadIdx.x / LANES; u < a.m * KB; u += 256 / LANES) {
       const int i = u / KB, kb = u % KB, lane = (int)threadIdx.x % LANES, k = kb * BLK + lane * 8, live = max(0, min(8, a.d - k));
       float v[8];
@@ -311,14 +311,17 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
         ld8n<TT_F16>(a.q, i * a.ldq + k, live, v);
       uint32_t byte;
       *reinterpret_cast<u32x2*>(enc + u * ROWB + lane * 8) = encode8(v, byte);
-      if (lane == 0) enc[16 * KB * ROWB + u] = (uint8_t)byte;
+      if (lane == 0) enc[16 * QT * KB * ROWB + u] = (uint8_t)byte;
     }
     __syncthreads();
-    const int row = min(r, (int)a.m - 1);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      b[kb][0] = row_frag(enc + (row * KB + kb) * ROWB, g);
-      sb[kb][0] = enc[16 * KB * ROWB + row * KB + kb];
+    for (int j = 0; j < QT; ++j) {
+      const int row = min(16 * j + r, (int)a.m - 1);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        b[kb][j] = row_frag(enc + (row * KB + kb) * ROWB, g);
+        sb[kb][j] = enc[16 * QT * KB * ROWB + row * KB + kb];
+      }
     }
   } else {
 #pragma unroll

@@ -195,9 +195,9 @@ def test_host_argument_errors():
                dict(d=0), dict(m=-2), dict(n=-1), dict(q=p + 1, dt=1), dict(out=p + 2), dict(codes=p + 8)):
         assert scores(**kw) == N.TT_ERR_ARG, kw
     assert L.tt_cat_scores_workspace_bytes(-1, 4, 8) == N.TT_ERR_ARG
-    need = L.tt_cat_scores_workspace_bytes(20, 4, 8)
-    assert need > 0 and scores(m=20, wsb=need - 1) == N.TT_ERR_WORKSPACE and scores(m=20, ws=None, wsb=need) == N.TT_ERR_ARG
-    assert scores(m=20, ws=p + 8, wsb=need) == N.TT_ERR_ARG
+    need = L.tt_cat_scores_workspace_bytes(70, 4, 8)
+    assert need > 0 and scores(m=70, wsb=need - 1) == N.TT_ERR_WORKSPACE and scores(m=70, ws=None, wsb=need) == N.TT_ERR_ARG
+    assert scores(m=70, ws=p + 8, wsb=need) == N.TT_ERR_ARG
     assert L.tt_cat_dq_workspace_bytes(4, 4, 0, 0) == N.TT_ERR_ARG
 
     def dq(ds=p, dt=0, m=2, lds=4, n=4, codes=p, scales=p, d=8, out=p, odt=0, ws=p, wsb=1 << 30):

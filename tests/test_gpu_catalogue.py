@@ -133,7 +133,8 @@ def check_dq(cat, q, ds, dq, n=None):
 
 
 SIZES = [(1, 1, 1), (1, 1000, 60), (2, 17, 128), (5, 3001, 256), (16, 64, 130), (17, 129, 512), (33, 515, 90), (64, 1000, 128),
-         (65, 66, 300), (100, 257, 1024), (129, 4099, 60), (300, 1025, 256), (513, 700, 129), (1030, 130, 64), (4, 70000, 33)]
+         (65, 66, 300), (100, 257, 1024), (129, 4099, 60), (300, 1025, 256), (513, 700, 129), (1030, 130, 64), (4, 70000, 33), (21, 300, 384),
+         (22, 300, 384), (32, 900, 256), (33, 900, 256), (16, 333, 512), (16, 333, 513), (50, 2000, 128)]
 
 
 @pytest.mark.parametrize("m,n,d", SIZES)
