@@ -2,9 +2,9 @@
 
 ``EmbeddingCatalogue`` keeps the rows that retrieval scores against (the CEO
 embeddings) in e4m3, in blocks of 128 values with a power-of-two scale: a
-quarter of the fp32 rows' bytes, and the product with a block of queries runs
-on the 8-bit matrix cores.  Rows are quantised as they are written and read
-back as the values they stand for.
+quarter of the fp32 rows' bytes.  Rows are quantised as they are written and
+read back as the values they stand for; the product with a block of queries is
+that of the values (exact in bfloat16, the matrix cores' operands).
 
     cat = EmbeddingCatalogue(n_ceos, 256, device="cuda")
     cat.write(ceo_embeddings)                    # rows 0, 1, ...
@@ -15,8 +15,9 @@ back as the values they stand for.
 Values: every rounding to e4m3 is to nearest even, off by at most 2^-4 of the
 value (2^-10 of the block's scale near zero).  Infinities and NaN are held as
 NaN and reach only the scores of their own row.  The queries are rounded the
-same way inside ``scores``; the gradient passes that rounding through unchanged
-and is ``ds @ read()`` with sums in 32 bits.  The catalogue itself gets no
+same way inside ``scores``, whose sums are in 32 bits and rounded once to the
+results' type; the gradient passes the queries' rounding through unchanged and
+is ``ds @ read()`` with sums in 32 bits.  The catalogue itself gets no
 gradient.
 
 On CPU tensors the same values come from torch ops.

@@ -4,9 +4,8 @@
 //
 // A power of two as scale makes every step but the rounding itself exact:
 // scaling moves the exponent only, a decoded e4m3 value times its scale is
-// exact in bfloat16 (4 significant bits), and the scaled MFMA takes the scale
-// byte as it is stored.  It costs up to one of e4m3's 17 binades of range, no
-// precision.
+// exact in bfloat16 (4 significant bits).  It costs up to one of e4m3's 17
+// binades of range, no precision.
 #pragma once
 #include "tt_common.h"
 

@@ -125,21 +125,18 @@ __global__ __launch_bounds__(256) void k_cat_read(const uint8_t* codes, const ui
 // operands, so this order of k is right; a load then takes 64 bytes of a row);
 // C: lane l holds C[row = 4 (l >> 4) + reg][column = l & 15].
 //
-// Results in 16 bits: v_mfma_scale_f32_16x16x128_f8f6f4, one instruction a
-// block, which takes both blocks' scale bytes, so the sums over all blocks
-// stay in the accumulator.  The 8-bit matrix instructions cut the products of
-// one instruction off below the largest of them (measured over all e4m3
-// values: a sum of 128 is off by up to 2^-11 of its largest product, 5e-5 of
-// the result in the 2-norm), far below the results' own rounding (2^-8, 2^-11)
-// but not a sum in 32 bits.
-// Results in 32 bits: both operands decoded to bf16, exactly, and
-// v_mfma_f32_16x16x32_bf16, whose sums measured 8e-8.
+// Both operands are decoded to bf16, exactly, for v_mfma_f32_16x16x32_bf16,
+// whose sums measured 8e-8 of the result in the 2-norm.  The 8-bit matrix
+// instructions, scaled ones and others, are no sums in 32 bits: they cut the
+// products of one instruction off below the largest of them (over all e4m3
+// values a sum of 128 is off by up to 2^-11 of its largest product, 5e-5 in the
+// 2-norm), which products that cancel leave in the result whatever its type.
+// They took 420 us where this takes 550 (8192 x 100000 x 256 in bf16), 17.6 /
+// 23.3 (513 x 20011 x 512), 39.1 / 41.8 (37 x 1000003 x 128), 277 / 271 (16384 x
+// 32771 x 128).
 // ---------------------------------------------------------------------------
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ f32x4 mfma_block8(const i32x8& a, const i32x8& b, const f32x4& c, int sa, int sb) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
-}
 // 8 codes and their block's scale -> bf16, exact
 __device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t lo, uint32_t hi, float s) {
   u32x4 w;
@@ -149,7 +146,7 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t lo, uint32_t hi, float 
   w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
   return __builtin_bit_cast(bf16x8, w);
 }
-__device__ __forceinline__ f32x4 mfma_block_bf16(const i32x8& a, const i32x8& b, f32x4 c, int sa, int sb) {
+__device__ __forceinline__ f32x4 mfma_block(const i32x8& a, const i32x8& b, f32x4 c, int sa, int sb) {
   const float fa = b8::scale_of((uint32_t)sa), fb = b8::scale_of((uint32_t)sb);
 #pragma unroll
   for (int h = 0; h < 4; ++h)
@@ -177,11 +174,6 @@ __device__ __forceinline__ i32x8 lds_frag(const uint8_t* s, int row, int g) {
 }
 // loads straight into LDS have arrived
 __device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-template <int DT>
-__device__ __forceinline__ f32x4 mfma_block(const i32x8& a, const i32x8& b, const f32x4& c, int sa, int sb) {
-  return DT == TT_F32 ? mfma_block_bf16(a, b, c, sa, sb) : mfma_block8(a, b, c, sa, sb);
-}
 
 // A wave's tile of 16 QT queries x 16 IT catalogue rows, stored row by row:
 // lane (r, g) holds 4 consecutive columns of row r; it is turned in the wave's
@@ -240,10 +232,11 @@ __device__ __forceinline__ void store_tile(uint8_t* so, const f32x4 (&acc)[IT][Q
 // in registers and walks over the catalogue, 16 IT rows at a time, straight
 // from global memory: no barrier, and the next rows' loads fly while this tile
 // is stored.  The 4 waves of a workgroup take neighbouring row groups, so that
-// a query's results go out in pieces of 64 IT values.  Measured: 1 x 1000003 x
-// 128 21.6 us (6.1 TB/s), 16 x 1000003 x 128 27 us (6.0 TB/s), 1 x 100000 x 256
-// 8.2 us.  For more queries the tiles below are faster (8192 x 100000 x 256: 776
-// against 420 us: every wave reads the catalogue through L2 again).
+// a query's results go out in pieces of 64 IT values.  Measured, calls back to
+// back (the codes stay in the last-level cache): 1 x 1000003 x 128 24.4 us, 16 x
+// 1000003 x 128 29.6 us, 1 x 100000 x 256 8.1 us.  For more queries the tiles below
+// are faster (8192 x 100000 x 256 on the 8-bit instructions: 776 against 420 us:
+// every wave reads the catalogue through L2 again).
 struct StreamArgs {
   const void* q;            // raw queries (ENC) or their codes
   const uint8_t* qs;        // their scale bytes (not ENC)
@@ -254,11 +247,13 @@ struct StreamArgs {
   int64_t panels, strips, per;  // workgroup t of an XCD's share: panel t / strips, strip t % strips
 };
 
-// NKB: blocks a row, 0: any number, with the queries' codes read again for every tile
-template <int DT, int IT, int QT, int NKB, bool ENC>
+// NKB: blocks a row, the queries encoded here and held in registers; 0: any number, with the queries' codes from the
+// workspace read again for every tile
+template <int DT, int IT, int QT, int NKB>
 __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs a) {
   using namespace b8;
-  constexpr int KB = NKB ? NKB : 1;
+  constexpr bool ENC = NKB > 0;
+  constexpr int KB = ENC ? NKB : 1;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * tile_lds<DT, IT, QT>()];
   __shared__ __attribute__((aligned(16))) uint8_t enc[ENC ? 16 * QT * KB * (ROWB + 1) : 16];  // ENC: the queries' codes, scale bytes
   const int l = lane_id(), w = wave_id(), r = l & 15, g = l >> 4;
@@ -267,7 +262,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   if (t >= a.panels * a.strips) return;
   const int64_t panel = t / a.strips, strip = t % a.strips;
   const int64_t m0 = panel * 16 * QT, n = a.n;
-  const int nkb = NKB ? NKB : a.nkb;
+  const int nkb = ENC ? NKB : a.nkb;
   // this strip's groups of 64 IT rows
   const int64_t groups = (n + 64 * IT - 1) / (64 * IT);
   const int64_t g0 = groups * strip / a.strips, g1 = groups * (strip + 1) / a.strips;
@@ -291,7 +286,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   };
   int64_t n0 = (g0 * 4 + w) * 16 * IT;
   const int64_t end = min(n, g1 * 64 * IT);
-  if (NKB > 0 && n0 < end) load(n0);
+  if (ENC && n0 < end) load(n0);
 
   const uint8_t* qrow[QT];
   const uint8_t* qsrow[QT];
@@ -299,7 +294,6 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   int sb[KB][QT];
   if constexpr (ENC) {
     // the workgroup encodes its queries once, 16 lanes a block
-    static_assert(NKB > 0, "the codes stay in registers");
     for (int u = (int)threadIdx.x / LANES; u < a.m * KB; u += 256 / LANES) {
       const int i = u / KB, kb = u % KB, lane = (int)threadIdx.x % LANES, k = kb * BLK + lane * 8, live = max(0, min(8, a.d - k));
       float v[8];
@@ -329,17 +323,10 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
       const int64_t at = min(m0 + 16 * j + r, a.m - 1);
       qrow[j] = (const uint8_t*)a.q + at * nkb * ROWB;
       qsrow[j] = a.qs + at * nkb;
-      if constexpr (NKB > 0) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          b[kb][j] = row_frag(qrow[j] + kb * ROWB, g);
-          sb[kb][j] = qsrow[j][kb];
-        }
-      }
     }
   }
 
-  if constexpr (NKB > 0) {
+  if constexpr (ENC) {
     f32x4 acc[IT][QT];
     auto multiply = [&]() {
 #pragma unroll
@@ -352,7 +339,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
         for (int i = 0; i < IT; ++i)
 #pragma unroll
           for (int j = 0; j < QT; ++j)
-            acc[i][j] = mfma_block<DT>(x[kb][i], b[kb][j], acc[i][j], sa[kb][i], sb[kb][j]);
+            acc[i][j] = mfma_block(x[kb][i], b[kb][j], acc[i][j], sa[kb][i], sb[kb][j]);
     };
     // whole tiles first; addresses of the one after the last stay inside the catalogue
     const int64_t whole = n * Elem<DT>::SIZE * 64 < 0x7FFFFFFF ? end - 16 * IT : -1;
@@ -398,7 +385,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
 #pragma unroll
         for (int i = 0; i < IT; ++i)
 #pragma unroll
-          for (int j = 0; j < QT; ++j) acc[i][j] = mfma_block<DT>(x[i], y[j], acc[i][j], sx[i], sy[j]);
+          for (int j = 0; j < QT; ++j) acc[i][j] = mfma_block(x[i], y[j], acc[i][j], sx[i], sy[j]);
       }
       store_tile<DT, IT, QT, false>(so, acc, a.out, m0, a.m, n0, n);
     }
@@ -424,10 +411,9 @@ __device__ __forceinline__ void store_wave(uint8_t* so, const f32x4 (&acc)[4][4]
 
 // Many queries: one workgroup a tile of 128 queries x 128 catalogue rows, a
 // wave 64 x 64 of it, a block of 128 values staged in LDS at a time.  Nothing is
-// fetched ahead: four workgroups a CU (128 registers a lane, 36 KB) cover each
-// other's loads and stores.  Two of 8 waves that keep 256 queries in registers
-// and stage ahead, with a quarter of the L2 reads, took 460 us where this takes
-// 420 (8192 x 100000 x 256 in bf16): their waves meet at barriers.
+// fetched ahead: three workgroups a CU (164 registers a lane, 36 KB) cover each
+// other's loads and stores (four, with 92 bytes a lane in scratch: 829 for 543 us
+// at 8192 x 100000 x 256 in bf16).
 constexpr int CT_M = 128, CT_N = 128;
 
 // Tile of workgroup `id` of 8 * per: XCD x runs workgroups x, x + 8, ... and
@@ -447,7 +433,7 @@ __device__ __forceinline__ bool cat_tile(int64_t id, int64_t per, int64_t mt, in
 }
 
 template <int DT>
-__global__ __launch_bounds__(256, DT == TT_F32 ? 3 : 4) void k_cat_scores(
+__global__ __launch_bounds__(256, 3) void k_cat_scores(
     const uint8_t* __restrict__ q, const uint8_t* __restrict__ qs, int64_t m, const uint8_t* __restrict__ codes,
     const uint8_t* __restrict__ scales, int64_t n, int nkb, void* out, int64_t mt, int64_t nt, int64_t per, int width) {
   using namespace b8;
@@ -504,7 +490,7 @@ __global__ __launch_bounds__(256, DT == TT_F32 ? 3 : 4) void k_cat_scores(
       const i32x8 b = lds_frag(sq, wm + 16 * j + r, g);
       const int sb = lds[2 * 128 * ROWB + 128 + wm + 16 * j + r];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i][j] = mfma_block<DT>(a[i], b, acc[i][j], sa[i], sb);
+      for (int i = 0; i < 4; ++i) acc[i][j] = mfma_block(a[i], b, acc[i][j], sa[i], sb);
     }
     __syncthreads();
   }
