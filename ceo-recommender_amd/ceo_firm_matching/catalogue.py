@@ -27,6 +27,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -36,6 +37,16 @@ from . import block8
 def _check_dtype(dtype: torch.dtype, what: str):
     if dtype not in N.DTYPES:
         raise NotImplementedError(f"{what}: float32, bfloat16 or float16, got {dtype}")
+
+
+# (without a Python frame where torch has it)
+_is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+
+
+def _check_traced(what: str):
+    """The kernels are launched on addresses: a traced graph would hold their empty results."""
+    if _is_tracing():
+        raise NotImplementedError(f"{what}: HIP kernels cannot be traced")
 
 
 def _rows_2d(x: torch.Tensor, d: int, what: str) -> torch.Tensor:
@@ -177,6 +188,8 @@ class EmbeddingCatalogue:
             self._check_range(start, m, "write")
         elif start:
             raise ValueError("write: rows or start, not both")
+        if self.device.type == "cuda":
+            _check_traced("write")
         if m == 0:
             return
         if not self.codes.is_inference():  # a backward that saved the old rows must notice
@@ -218,6 +231,7 @@ class EmbeddingCatalogue:
             out = torch.zeros(m, self.dim)
             out[ok] = block8.decode(self.codes[rows[ok]], self.scales[rows[ok]], self.dim)
             return out.to(dtype)
+        _check_traced("read")
         with N.on_device(self.device):
             out = torch.empty(m, self.dim, dtype=dtype, device=self.device)
             N.check(N.lib().tt_cat_read(self.codes.data_ptr(), self.scales.data_ptr(), self.capacity, self.dim,
@@ -229,7 +243,7 @@ class EmbeddingCatalogue:
                dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """Inner products of ``queries`` [..., dim] with the first ``count``
         rows (default: all), [..., count], in ``dtype`` (default: the
-        queries').  Differentiable in the queries."""
+        queries').  Differentiable in the queries, once, in reverse mode."""
         dtype = queries.dtype if dtype is None else dtype
         _check_dtype(queries.dtype, "scores")
         _check_dtype(dtype, "scores")
@@ -237,6 +251,10 @@ class EmbeddingCatalogue:
             raise ValueError(f"scores: queries on {queries.device}, the catalogue on {self.device}")
         if queries.dim() < 1 or queries.shape[-1] != self.dim:
             raise ValueError(f"scores: expected [..., {self.dim}], got {tuple(queries.shape)}")
+        if unpack_dual(queries).tangent is not None:
+            raise NotImplementedError("scores: no forward-mode derivative, use backward")
+        if self.device.type == "cuda":
+            _check_traced("scores")
         n = self.capacity if count is None else int(count)
         self._check_range(0, n, "scores")
         flat = queries.dim() == 2
