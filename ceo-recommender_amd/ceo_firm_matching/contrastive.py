@@ -410,11 +410,12 @@ def retrieval_ranks(firm_emb: torch.Tensor, ceo_emb: torch.Tensor, cap: Optional
     if storage not in (None, "e4m3"):
         raise ValueError(f"retrieval_ranks: storage is None or 'e4m3', got {storage!r}")
     N_ = firm_emb.size(0) if cap is None else min(firm_emb.size(0), cap)
+    f, c = firm_emb[:N_], ceo_emb[:N_]
     if storage is None:
-        return retrieval_ranks_rows(firm_emb[:N_], ceo_emb[:N_], 0)
-    catalogue = EmbeddingCatalogue(N_, ceo_emb.shape[1], device=ceo_emb.device)
-    catalogue.write(ceo_emb[:N_])
-    return catalogue_ranks(firm_emb[:N_], catalogue)
+        return retrieval_ranks_rows(f, c, 0)
+    catalogue = EmbeddingCatalogue(c.shape[0], c.shape[1], device=c.device)
+    catalogue.write(c)
+    return catalogue_ranks(f, catalogue)
 
 
 def metrics_from_ranks(ranks: torch.Tensor, top_k: int = 10) -> Dict[str, float]:
