@@ -124,6 +124,15 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"Invalid weight_decay value: {g['weight_decay']}")
 
     @staticmethod
+    def _check_options(g):
+        """Options of torch's optimizers under which its step is another one."""
+        for option in ("maximize", "amsgrad", "differentiable"):
+            if g.get(option):
+                raise NotImplementedError(f"AdamW: {option}={g[option]} is not supported")
+        if not g.get("decoupled_weight_decay", True) and g["weight_decay"] != 0:
+            raise NotImplementedError("AdamW: weight decay that is added to the gradient is not supported")
+
+    @staticmethod
     def _check_apart(params):
         """One launch updates all of them: no value may be in two."""
         at = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
@@ -135,6 +144,7 @@ class AdamW(torch.optim.Optimizer):
         g = self.param_groups[-1]
         try:
             self._check_hyper(g)
+            self._check_options(g)
             for p in g["params"]:
                 if p.dtype not in N.DTYPES:
                     raise NotImplementedError(f"AdamW: float32, bfloat16 or float16 parameters, got {p.dtype}")
@@ -266,9 +276,20 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Hyperparameters and states, copied into the arenas that the steps
         (captured ones too) already use.  8-bit states load from 8-bit ones
-        only; 32-bit ones also from ``torch.optim.AdamW``'s."""
+        only; 32-bit ones also from ``torch.optim.AdamW``'s.  Options that
+        this step does not follow (``maximize``, ``amsgrad``,
+        ``differentiable``, a decay that is not decoupled) are refused, and
+        nothing has changed then."""
         given = state_dict["state"]
-        ids = list(chain.from_iterable(g["params"] for g in state_dict["param_groups"]))
+        groups = []
+        for g in state_dict["param_groups"]:
+            g = dict(g)
+            g.update({k: float(g[k]) for k in ("lr", "eps", "weight_decay")}, betas=tuple(map(float, g["betas"])))  # (tensors too)
+            self._check_hyper(g)
+            self._check_options(g)
+            g.pop("decoupled_weight_decay", None)
+            groups.append(g)
+        ids = list(chain.from_iterable(g["params"] for g in groups))
         mine = list(chain.from_iterable(g["params"] for g in self.param_groups))
         if len(ids) == len(mine):  # (another count is the base class's error)
             for k, p in zip(ids, mine):
@@ -281,7 +302,7 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError(f"AdamW: state {name!r} is {tuple(a.shape)} {a.dtype}, "
                                          f"expected {tuple(to.shape)} {to.dtype}")
         keep = self.state
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        super().load_state_dict({"state": {}, "param_groups": groups})
         self.state = keep
         with torch.no_grad():
             for k, p in zip(ids, mine):
