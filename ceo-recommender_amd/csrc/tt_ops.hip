@@ -47,8 +47,9 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
                       const tt_adamw_state* state, const tt_adamw_hp* hp, uint64_t seed, tt_stream_t stream) {
   if (!state || !hp || n_tensors < 0 || (n_tensors > 0 && !tensors)) return TT_ERR_ARG;
   if (state_bits != 8 && state_bits != 32) return TT_ERR_UNSUPPORTED;
-  if (!(hp->beta1 >= 0.0 && hp->beta1 < 1.0 && hp->beta2 >= 0.0 && hp->beta2 < 1.0 && hp->eps >= 0.0)) return TT_ERR_ARG;
-  if (!std::isfinite(hp->lr) || !std::isfinite(hp->weight_decay)) return TT_ERR_ARG;
+  if (!(hp->beta1 >= 0.0 && hp->beta1 < 1.0 && hp->beta2 >= 0.0 && hp->beta2 < 1.0)) return TT_ERR_ARG;
+  for (const double x : {hp->lr, hp->eps, hp->weight_decay})
+    if (!(x >= 0.0) || !std::isfinite(x)) return TT_ERR_ARG;
   if (state->n_blocks < 0 || state->n_blocks > (int64_t)UINT32_MAX) return TT_ERR_ARG;  // the hash takes 32 bits
   if (state->steps && !state->coefs) return TT_ERR_ARG;
   int64_t values = 0;

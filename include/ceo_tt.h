@@ -511,7 +511,7 @@ typedef struct tt_adamw_state {
   int64_t n_steps;
 } tt_adamw_state;
 typedef struct tt_adamw_hp {
-  double lr, beta1, beta2, eps, weight_decay;
+  double lr, beta1, beta2, eps, weight_decay;   /* finite, >= 0; beta1, beta2 < 1 */
 } tt_adamw_hp;
 int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t state_bits,
                       const tt_adamw_state* state, const tt_adamw_hp* hp, uint64_t seed,
