@@ -67,23 +67,40 @@ struct AdamwHp {
   float w1, b2, c2, eps, decay;
 };
 
-// p, m, v in; p', m', v' out; returns sqrt(v').  FAST (8-bit states, whose
-// kernel the instructions bound): the hardware's square root and reciprocal,
-// off by one unit in the last place each, for the correctly rounded ones of
-// about 12 instructions.
-template <bool FAST>
-__device__ __forceinline__ float adamw_elem(float& p, float& m, float& v, float g, const AdamwHp& h,
-                                            const AdamwCoef& c, float inv_bc2s) {
+__device__ __forceinline__ void adamw_moments(float& m, float& v, float g, const AdamwHp& h) {
   m = m + h.w1 * (g - m);
   v = v * h.b2 + (h.c2 * g) * g;
-  if constexpr (FAST) {
-    const float r = __builtin_amdgcn_sqrtf(v);
-    p = p * h.decay - c.step_size * (m * __builtin_amdgcn_rcpf(r * inv_bc2s + h.eps));
-    return r;
+}
+// 32-bit states: correctly rounded root and quotients
+__device__ __forceinline__ void adamw_elem(float& p, float& m, float& v, float g, const AdamwHp& h, const AdamwCoef& c) {
+  adamw_moments(m, v, g, h);
+  p = p * h.decay - c.step_size * (m / (sqrtf(v) / c.bc2s + h.eps));
+}
+
+// Roots of a thread's 8 values of v' (8-bit states, whose kernel the
+// instructions bound): the hardware's square root, off by one unit in the last
+// place, for the correctly rounded one of about 12 instructions; the same for
+// the reciprocal in the update.  The hardware takes subnormal input as zero, so
+// a wave that holds such values takes their roots of v' 2^64.
+__device__ __forceinline__ void roots8(const float (&v)[8], float (&r)[8]) {
+  uint32_t least = ~0u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    r[e] = __builtin_amdgcn_sqrtf(v[e]);
+    least = min(least, __float_as_uint(v[e]));
   }
-  const float r = sqrtf(v);
-  p = p * h.decay - c.step_size * (m / (r / c.bc2s + h.eps));
-  return r;
+  if (__ballot(least < 0x00800000u)) {
+    asm volatile("");  // a branch: zeros are common, subnormals are not
+    least = ~0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) least = min(least, __float_as_uint(v[e]) - 1u);  // zero goes to the top
+    if (__ballot(least < 0x007FFFFFu)) {
+      asm volatile("");
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (__float_as_uint(v[e]) < 0x00800000u) r[e] = __builtin_amdgcn_sqrtf(v[e] * 0x1p64f) * 0x1p-32f;
+    }
+  }
 }
 
 // whether a byte of w is 0xFF (and at times where one is 0xFE below a 0xFF: never without one)
@@ -115,7 +132,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamwArgs& a, int k, const Ada
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) adamw_elem<false>(p[q][e], m[q][e], v[q][e], g[q][e], h, c, 0.f);
+        for (int e = 0; e < PER; ++e) adamw_elem(p[q][e], m[q][e], v[q][e], g[q][e], h, c);
         stv<DT, PER>(P, i + q * HALF, p[q]);
         stv<TT_F32, PER>(a.m, blk0 * BLK + i + q * HALF, m[q]);
         stv<TT_F32, PER>(a.v, blk0 * BLK + i + q * HALF, v[q]);
@@ -129,7 +146,7 @@ __device__ __forceinline__ void adamw_chunk(const AdamwArgs& a, int k, const Ada
       ldn<TT_F32, PER>(a.m, blk0 * BLK + i, live, m);
       ldn<TT_F32, PER>(a.v, blk0 * BLK + i, live, v);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) adamw_elem<false>(p[e], m[e], v[e], g[e], h, c, 0.f);
+      for (int e = 0; e < PER; ++e) adamw_elem(p[e], m[e], v[e], g[e], h, c);
       stn<DT, PER>(P, i, live, p);
       stn<TT_F32, PER>(a.m, blk0 * BLK + i, live, m);  // (the padding stays zero)
       stn<TT_F32, PER>(a.v, blk0 * BLK + i, live, v);
@@ -162,11 +179,16 @@ __device__ __forceinline__ void adamw_chunk(const AdamwArgs& a, int k, const Ada
         for (int e = 0; e < 8; ++e)
           if (((rc[e / 4] >> (8 * (e % 4))) & 0xFFu) == NAN_R) root[e] = __uint_as_float(0x7FC00000u);
       }
-      uint32_t am = 0, ar = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[e] = root[e] * root[e];
-        r[e] = adamw_elem<true>(p[e], m[e], v[e], g[e], h, c, inv_bc2s);
+        adamw_moments(m[e], v[e], g[e], h);
+      }
+      roots8(v, r);
+      uint32_t am = 0, ar = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = p[e] * h.decay - c.step_size * (m[e] * __builtin_amdgcn_rcpf(r[e] * inv_bc2s + h.eps));
         am = max(am, __float_as_uint(m[e]) & 0x7FFFFFFFu);
         ar = max(ar, __float_as_uint(r[e]));  // a root's sign bit is a NaN's
       }
