@@ -47,20 +47,25 @@ struct AdamwArgs {
   float w1, b2, c2, eps, decay;
   float *m, *v;
   uint8_t *mc, *ms, *rc, *rs;
-  int64_t* steps;
-  AdamwCoef* coefs;
-  double lr, b1d, b2d;
-  uint64_t seed;
+  const AdamwCoef* coefs;      // device steps, or null
 };
 static_assert(sizeof(AdamwArgs) <= 4096, "kernel arguments");
 
-// device step counters: one thread a tensor, before k_adamw
-__global__ __launch_bounds__(ADAMW_LIST) void k_adamw_advance(AdamwArgs a) {
+// device step counters: one thread a counter, each named once, before any k_adamw of the call
+struct AdamwCounters {
+  int64_t* steps;
+  AdamwCoef* coefs;
+  double lr, b1, b2;
+  uint64_t seed;
+  uint32_t at[ADAMW_LIST];
+  int32_t n;
+};
+__global__ __launch_bounds__(ADAMW_LIST) void k_adamw_advance(AdamwCounters a) {
   const int k = (int)threadIdx.x;
-  if (k >= a.n_t) return;
-  const uint32_t i = a.c[k].key_lo;
+  if (k >= a.n) return;
+  const uint32_t i = a.at[k];
   const int64_t t = ++a.steps[i];
-  a.coefs[i] = adamw_coef(a.lr, a.b1d, a.b2d, a.seed, t);
+  a.coefs[i] = adamw_coef(a.lr, a.b1, a.b2, a.seed, t);
 }
 
 struct AdamwHp {
@@ -244,7 +249,7 @@ __global__ __launch_bounds__(ADAMW_THREADS) void k_adamw(AdamwArgs a) {
   const uint64_t le = __ballot(a.first[lane_id()] <= (int32_t)blockIdx.x);
   const int k = __builtin_amdgcn_readfirstlane(__popcll(le) - 1);
   const int64_t from = (int64_t)((int32_t)blockIdx.x - a.first[k]) * a.chunk;
-  const AdamwCoef c = a.steps ? a.coefs[a.c[k].key_lo] : a.c[k];
+  const AdamwCoef c = a.coefs ? a.coefs[a.c[k].key_lo] : a.c[k];
   switch (a.dtype[k]) {
     case TT_F32: adamw_chunk<BITS, TT_F32>(a, k, c, from); break;
     case TT_BF16: adamw_chunk<BITS, TT_BF16>(a, k, c, from); break;

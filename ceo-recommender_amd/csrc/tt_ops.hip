@@ -4,6 +4,8 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <memory>
+#include <new>
 #include <type_traits>
 
 #include "tt_adamw.hip"
@@ -37,6 +39,37 @@ static void with_dtype(int32_t dt, F f) {
     f(std::integral_constant<int, TT_F16>{});
 }
 
+// Raises every counter that the list names, once each.  Rising indices (one a
+// tensor) go out as they come, others are sorted first.
+static int adamw_advance(const tt_adamw_tensor* tensors, int32_t n, const tt_adamw_state& st, const tt_adamw_hp& hp,
+                         uint64_t seed, hipStream_t s) {
+  AdamwCounters a{st.steps, (AdamwCoef*)st.coefs, hp.lr, hp.beta1, hp.beta2, seed, {}, 0};
+  bool rising = true;
+  int64_t last = -1;
+  for (int32_t i = 0; i < n; ++i) {
+    if (tensors[i].n == 0) continue;
+    rising = rising && tensors[i].step > last;
+    last = tensors[i].step;
+  }
+  std::unique_ptr<uint32_t[]> sorted;
+  int32_t count = n;
+  if (!rising) {
+    sorted.reset(new (std::nothrow) uint32_t[n]);
+    if (!sorted) return (int)hipErrorOutOfMemory;
+    count = 0;
+    for (int32_t i = 0; i < n; ++i)
+      if (tensors[i].n) sorted[count++] = (uint32_t)tensors[i].step;
+    std::sort(sorted.get(), sorted.get() + count);
+    count = (int32_t)(std::unique(sorted.get(), sorted.get() + count) - sorted.get());
+  }
+  for (int32_t i = 0; i < count;) {
+    for (a.n = 0; i < count && a.n < ADAMW_LIST; ++i)
+      if (sorted || tensors[i].n) a.at[a.n++] = sorted ? sorted[i] : (uint32_t)tensors[i].step;
+    if (a.n) hipLaunchKernelGGL(k_adamw_advance, dim3(1), dim3(ADAMW_LIST), 0, s, a);
+  }
+  return ops_launch_check();
+}
+
 }  // namespace tt
 
 using namespace tt;
@@ -51,7 +84,7 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
   for (const double x : {hp->lr, hp->eps, hp->weight_decay})
     if (!(x >= 0.0) || !std::isfinite(x)) return TT_ERR_ARG;
   if (state->n_blocks < 0 || state->n_blocks > (int64_t)UINT32_MAX) return TT_ERR_ARG;  // the hash takes 32 bits
-  if (state->steps && !state->coefs) return TT_ERR_ARG;
+  if (state->steps && (!state->coefs || state->n_steps > (int64_t)UINT32_MAX)) return TT_ERR_ARG;
   int64_t values = 0;
   for (int32_t i = 0; i < n_tensors; ++i) {
     const tt_adamw_tensor& t = tensors[i];
@@ -83,12 +116,9 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
   a.ms = state->m_scales;
   a.rc = state->r_codes;
   a.rs = state->r_scales;
-  a.steps = state->steps;
-  a.coefs = (AdamwCoef*)state->coefs;
-  a.lr = hp->lr;
-  a.b1d = hp->beta1;
-  a.b2d = hp->beta2;
-  a.seed = seed;
+  a.coefs = state->steps ? (const AdamwCoef*)state->coefs : nullptr;
+  if (state->steps)
+    if (const int rc = adamw_advance(tensors, n_tensors, *state, *hp, seed, s)) return rc;
   // 8-bit states of many values: 4 rounds a workgroup spare three of four looks for its tensor (96 M values in bf16:
   // 292 -> 239 us; 32-bit states 517 -> 528 us, small lists want the workgroups)
   const int64_t chunk = ADAMW_STRIDE * (state_bits == 8 && values >= 1 << 22 ? 4 : 1);
@@ -121,7 +151,6 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
     if (a.n_t == 0) break;
     for (int k = a.n_t; k < ADAMW_LIST; ++k) a.first[k] = INT32_MAX;
     a.chunk = (int32_t)chunk;
-    if (state->steps) hipLaunchKernelGGL(k_adamw_advance, dim3(1), dim3(ADAMW_LIST), 0, s, a);
     if (state_bits == 32)
       hipLaunchKernelGGL(k_adamw<32>, dim3((unsigned)chunks), dim3(ADAMW_THREADS), 0, s, a);
     else
