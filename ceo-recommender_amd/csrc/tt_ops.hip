@@ -47,7 +47,6 @@ static int adamw_advance(const tt_adamw_tensor* tensors, int32_t n, const tt_ada
   bool rising = true;
   int64_t last = -1;
   for (int32_t i = 0; i < n; ++i) {
-    if (tensors[i].n == 0) continue;
     rising = rising && tensors[i].step > last;
     last = tensors[i].step;
   }
@@ -56,16 +55,13 @@ static int adamw_advance(const tt_adamw_tensor* tensors, int32_t n, const tt_ada
   if (!rising) {
     sorted.reset(new (std::nothrow) uint32_t[n]);
     if (!sorted) return (int)hipErrorOutOfMemory;
-    count = 0;
-    for (int32_t i = 0; i < n; ++i)
-      if (tensors[i].n) sorted[count++] = (uint32_t)tensors[i].step;
-    std::sort(sorted.get(), sorted.get() + count);
-    count = (int32_t)(std::unique(sorted.get(), sorted.get() + count) - sorted.get());
+    for (int32_t i = 0; i < n; ++i) sorted[i] = (uint32_t)tensors[i].step;
+    std::sort(sorted.get(), sorted.get() + n);
+    count = (int32_t)(std::unique(sorted.get(), sorted.get() + n) - sorted.get());
   }
   for (int32_t i = 0; i < count;) {
-    for (a.n = 0; i < count && a.n < ADAMW_LIST; ++i)
-      if (sorted || tensors[i].n) a.at[a.n++] = sorted ? sorted[i] : (uint32_t)tensors[i].step;
-    if (a.n) hipLaunchKernelGGL(k_adamw_advance, dim3(1), dim3(ADAMW_LIST), 0, s, a);
+    for (a.n = 0; i < count && a.n < ADAMW_LIST; ++i) a.at[a.n++] = sorted ? sorted[i] : (uint32_t)tensors[i].step;
+    hipLaunchKernelGGL(k_adamw_advance, dim3(1), dim3(ADAMW_LIST), 0, s, a);
   }
   return ops_launch_check();
 }
@@ -89,17 +85,17 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
   for (int32_t i = 0; i < n_tensors; ++i) {
     const tt_adamw_tensor& t = tensors[i];
     if (t.n < 0 || !dtype_ok(t.dtype)) return TT_ERR_ARG;
-    if (t.n == 0) continue;
+    if (state->steps && (t.step < 0 || t.step >= state->n_steps)) return TT_ERR_ARG;
+    if (t.n == 0) continue;  // its counter still counts
     const uintptr_t es = size_of((int32_t)t.dtype);
     if (!t.param || !t.grad || !aligned(t.param, es) || !aligned(t.grad, es)) return TT_ERR_ARG;
     const int64_t nb = (t.n - 1) / TT_BLOCK + 1;
     if (t.block0 < 0 || nb > state->n_blocks || t.block0 > state->n_blocks - nb) return TT_ERR_ARG;
-    if (state->steps ? t.step < 0 || t.step >= state->n_steps : t.step < 1) return TT_ERR_ARG;
+    if (!state->steps && t.step < 1) return TT_ERR_ARG;
     values += t.n;
   }
-  if (values == 0) return TT_OK;
-  if (state_bits == 32 ? !state->exp_avg || !state->exp_avg_sq
-                       : !state->m_codes || !state->m_scales || !state->r_codes || !state->r_scales)
+  if (values > 0 && (state_bits == 32 ? !state->exp_avg || !state->exp_avg_sq
+                                      : !state->m_codes || !state->m_scales || !state->r_codes || !state->r_scales))
     return TT_ERR_ARG;
   if (!aligned(state->exp_avg, 4) || !aligned(state->exp_avg_sq, 4) || !aligned(state->steps, 8) || !aligned(state->coefs, 4))
     return TT_ERR_ARG;
@@ -119,6 +115,7 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
   a.coefs = state->steps ? (const AdamwCoef*)state->coefs : nullptr;
   if (state->steps)
     if (const int rc = adamw_advance(tensors, n_tensors, *state, *hp, seed, s)) return rc;
+  if (values == 0) return TT_OK;
   // 8-bit states of many values: 4 rounds a workgroup spare three of four looks for its tensor (96 M values in bf16:
   // 292 -> 239 us; 32-bit states 517 -> 528 us, small lists want the workgroups)
   const int64_t chunk = ADAMW_STRIDE * (state_bits == 8 && values >= 1 << 22 ? 4 : 1);

@@ -489,8 +489,8 @@ int32_t tt_train_step_dp(const tt_model_desc* d, float* params, float* buffers, 
  *     infinities and NaN are held as NaN.
  * t = tensors[i].step, or with `steps` (device int64, capturable): that
  * entry's counter steps[tensors[i].step].  The call raises each counter that
- * the list names by one, however many tensors share it, before any of them
- * takes its step.                                                           */
+ * the list names by one, however many tensors share it (empty ones too),
+ * before any of them takes its step.                                        */
 #define TT_BLOCK 128
 #define TT_F32 0
 #define TT_BF16 1

@@ -84,3 +84,25 @@ def test_refusals():
         assert a.step() == N.TT_ERR_ARG, field
     a = Lists([10, 20], [0, -1], 2, 32, cpu)
     assert a.step() == N.TT_ERR_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("shapes", [[(0, 4)], [(0, 4), (5,), (0,)], [(3,)] * 70 + [(0,)]])
+def test_empty_parameters_count_their_steps(dev, bits, shapes):
+    """As with step counts on the host."""
+    counts = []
+    for capturable in (False, True):
+        params = [torch.nn.Parameter(torch.ones(s, device=dev)) for s in shapes]
+        opt = AdamW(params, state_bits=bits, capturable=capturable)
+        for _ in range(2):
+            for p in params:
+                p.grad = torch.ones_like(p)
+            opt.step()
+        counts.append([int(opt.state[p]["step"]) for p in params])
+    assert counts[0] == counts[1] == [2] * len(shapes)
+
+
+def test_the_counter_of_an_empty_tensor_is_checked():
+    a = Lists([10, 0], [0, 7], 2, 32, torch.device("cpu"))
+    assert a.step() == N.TT_ERR_ARG
