@@ -238,7 +238,7 @@ class AdamW(torch.optim.Optimizer):
                 mc, ms, rc, rs = (b.arenas[k][at] for k in _BYTES)
                 m = block8.held(mc, ms, block8.E4M3)
                 v = block8.held(rc, rs, block8.E4M4).square()
-            m = m + (1 - b1) * (gf - m)
+            m = gf - b1 * (gf - m) if b1 < 0.5 else m + (1 - b1) * (gf - m)
             v = b2 * v + (1 - b2) * gf * gf
             r = v.sqrt()
             x = x * (1 - g["lr"] * g["weight_decay"]) - (g["lr"] / (1 - b1 ** t)) * (m / (r / (1 - b2 ** t) ** 0.5 + g["eps"]))

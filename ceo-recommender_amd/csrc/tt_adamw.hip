@@ -1,6 +1,7 @@
 // AdamW over a list of tensors (gfx950), states in 32 or in 8 bits.
 //
-//   m' = m + (1 - b1)(g - m);  v' = b2 v + (1 - b2) g^2
+//   m' = m + (1 - b1)(g - m), for b1 < 1/2 g - b1 (g - m): the rounding of g - m
+//   by the smaller factor;  v' = b2 v + (1 - b2) g^2
 //   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
 // k_adamw takes up to ADAMW_LIST tensors by value (kernel arguments, so a
@@ -44,7 +45,8 @@ struct AdamwArgs {
   int32_t first[ADAMW_LIST];   // first chunk of the tensor; INT32_MAX past the list
   int32_t chunk;               // values per chunk, a multiple of ADAMW_STRIDE
   int32_t n_t;
-  float w1, b2, c2, eps, decay;
+  float w1, b2, c2, eps, decay;  // w1: 1 - b1, or -b1 with from_grad
+  int32_t from_grad;
   float *m, *v;
   uint8_t *mc, *ms, *rc, *rs;
   const AdamwCoef* coefs;      // device steps, or null
@@ -70,10 +72,11 @@ __global__ __launch_bounds__(ADAMW_LIST) void k_adamw_advance(AdamwCounters a) {
 
 struct AdamwHp {
   float w1, b2, c2, eps, decay;
+  bool from_grad;
 };
 
 __device__ __forceinline__ void adamw_moments(float& m, float& v, float g, const AdamwHp& h) {
-  m = m + h.w1 * (g - m);
+  m = (h.from_grad ? g : m) + h.w1 * (g - m);
   v = v * h.b2 + (h.c2 * g) * g;
 }
 // 32-bit states: correctly rounded root and quotients
@@ -114,7 +117,7 @@ __device__ __forceinline__ bool has_ff(uint32_t w) { return ((~w - 0x01010101u) 
 template <int BITS, int DT>
 __device__ __forceinline__ void adamw_chunk(const AdamwArgs& a, int k, const AdamwCoef& c, int64_t from) {
   using namespace b8;
-  const AdamwHp h{a.w1, a.b2, a.c2, a.eps, a.decay};
+  const AdamwHp h{a.w1, a.b2, a.c2, a.eps, a.decay, a.from_grad != 0};
   void* const P = a.p[k];
   const void* const G = a.g[k];
   const int64_t n = a.n[k], blk0 = a.blk[k];

@@ -101,7 +101,8 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
     return TT_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   AdamwArgs a;
-  a.w1 = (float)(1.0 - hp->beta1);
+  a.from_grad = hp->beta1 < 0.5;
+  a.w1 = (float)(a.from_grad ? -hp->beta1 : 1.0 - hp->beta1);
   a.b2 = (float)hp->beta2;
   a.c2 = (float)(1.0 - hp->beta2);
   a.eps = (float)hp->eps;

@@ -475,7 +475,7 @@ int32_t tt_train_step_dp(const tt_model_desc* d, float* params, float* buffers, 
 /* ---- AdamW over many tensors (ABI 7) --------------------------------------
  * One decoupled-weight-decay Adam step over a list of tensors of any sizes in
  * one launch per 64 tensors, beside tt_adam_apply's one flat arena:
- *   m' = m + (1 - b1)(g - m);  v' = b2 v + (1 - b2) g^2;
+ *   m' = b1 m + (1 - b1) g;  v' = b2 v + (1 - b2) g^2;
  *   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
  * in 32 bits whatever the tensors' type, p' rounded once.  The states live in
  * arenas of blocks of TT_BLOCK values: tensor i's values start at block
