@@ -175,6 +175,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        steps = []  # every group is checked before the first one steps
         for g, b in zip(self.param_groups, self._buckets):
             live, params, grads = None, b.params, list(map(_grad, b.params))
             try:
@@ -196,17 +197,26 @@ class AdamW(torch.optim.Optimizer):
                 if any(x.layout != torch.strided for x in grads):
                     raise NotImplementedError("AdamW: sparse gradients are not supported")
                 grads = [x.contiguous() for x in grads]
+            if b.device.type != "cuda" or len(self._buckets) > 1:  # (a single HIP group's step checks them itself)
+                self._check_hyper(g)
+                if b.device.type == "cuda":
+                    with N.on_device(b.device):
+                        self._check_capture()
+            steps.append((g, b, live, params, grads))
+        for g, b, live, params, grads in steps:
             if b.device.type == "cuda":
                 self._step_hip(g, b, live, params, grads)
             else:
-                self._check_hyper(g)
                 self._step_cpu(g, b, range(len(params)) if live is None else live, grads)
         return loss
 
+    def _check_capture(self):
+        if not self._capturable and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a captured step needs capturable=True (the step count would be frozen)")
+
     def _step_hip(self, g, b, live, params, grads):
         with N.on_device(b.device):
-            if not self._capturable and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdamW: a captured step needs capturable=True (the step count would be frozen)")
+            self._check_capture()
             t, at = (b.table, b.table_at) if live is None else (b.table[live], 0)
             t[:, 0] = list(map(_address, params))
             t[:, 1] = list(map(_address, grads))
