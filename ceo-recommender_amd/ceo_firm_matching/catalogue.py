@@ -27,7 +27,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -251,7 +251,8 @@ class EmbeddingCatalogue:
             raise ValueError(f"scores: queries on {queries.device}, the catalogue on {self.device}")
         if queries.dim() < 1 or queries.shape[-1] != self.dim:
             raise ValueError(f"scores: expected [..., {self.dim}], got {tuple(queries.shape)}")
-        if unpack_dual(queries).tangent is not None:
+        # (outside every dual level, known without a call, there is no tangent)
+        if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(queries).tangent is not None:
             raise NotImplementedError("scores: no forward-mode derivative, use backward")
         if self.device.type == "cuda":
             _check_traced("scores")
