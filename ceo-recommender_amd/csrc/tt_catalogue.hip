@@ -207,15 +207,17 @@ __device__ __forceinline__ void store_tile(uint8_t* so, const f32x4 (&acc)[IT][Q
   uint8_t* const base = (uint8_t*)out + (m0 * n + n0) * ES;
 #pragma unroll
   for (int k = 0; k < (16 * QT * LPR + 63) / 64; ++k) {
-    const int u = k * 64 + l, row = u / LPR, c = (u % LPR) * PER;
+    const int u = k * 64 + l;
+    const bool piece = 16 * QT * LPR % 64 == 0 || u < 16 * QT * LPR;
+    const int row = piece ? u / LPR : 0, c = (u % LPR) * PER;
     const uint8_t* from = so + row * LDO + c * ES;
     if constexpr (WHOLE) {
       // no branch: the loop over tiles then knows how many stores follow the
       // next tile's loads and waits for the loads alone
-      const uint32_t off = row < rows && u < 16 * QT * LPR ? (uint32_t)row * (uint32_t)(n * ES) + (uint32_t)(c * ES) : 0x80000000u;
+      const uint32_t off = piece && row < rows ? (uint32_t)row * (uint32_t)(n * ES) + (uint32_t)(c * ES) : 0x80000000u;
       const auto rs = __builtin_amdgcn_make_buffer_rsrc(base, (short)0, 0x7FFFFFFF, 0x00020000);
       __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4*>(from), rs, (int)off, 0, 0);
-    } else if (row < rows && c < cols) {
+    } else if (piece && row < rows && c < cols) {
       uint8_t* to = base + ((int64_t)row * n + c) * ES;
       if (c + PER <= cols) {
         const u32x4 v = *reinterpret_cast<const u32x4*>(from);
