@@ -246,7 +246,7 @@ struct StreamArgs {
   void* out;
   int64_t m, n, ldq;
   int d, nkb, q_dtype;
-  int64_t panels, strips, per;  // workgroup t of an XCD's share: panel t / strips, strip t % strips
+  int64_t strips, per;          // workgroups; those of an XCD
 };
 
 // NKB: blocks a row, the queries encoded here and held in registers; 0: any number, with the queries' codes from the
@@ -260,10 +260,9 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   __shared__ __attribute__((aligned(16))) uint8_t enc[ENC ? 16 * QT * KB * (ROWB + 1) : 16];  // ENC: the queries' codes, scale bytes
   const int l = lane_id(), w = wave_id(), r = l & 15, g = l >> 4;
   uint8_t* const so = lds + w * tile_lds<DT, IT, QT>();
-  const int64_t t = (int64_t)(blockIdx.x & 7) * a.per + (blockIdx.x >> 3);
-  if (t >= a.panels * a.strips) return;
-  const int64_t panel = t / a.strips, strip = t % a.strips;
-  const int64_t m0 = panel * 16 * QT, n = a.n;
+  const int64_t strip = (int64_t)(blockIdx.x & 7) * a.per + (blockIdx.x >> 3);
+  if (strip >= a.strips) return;
+  const int64_t n = a.n;
   const int nkb = ENC ? NKB : a.nkb;
   // this strip's groups of 64 IT rows
   const int64_t groups = (n + 64 * IT - 1) / (64 * IT);
@@ -322,7 +321,7 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
   } else {
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
-      const int64_t at = min(m0 + 16 * j + r, a.m - 1);
+      const int64_t at = min((int64_t)(16 * j + r), a.m - 1);
       qrow[j] = (const uint8_t*)a.q + at * nkb * ROWB;
       qsrow[j] = a.qs + at * nkb;
     }
@@ -350,11 +349,11 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
       const int64_t at = n0;
       n0 += 64 * IT;
       load(min(n0, n - 1));  // in flight while this tile is stored
-      store_tile<DT, IT, QT, true>(so, acc, a.out, m0, a.m, at, n);
+      store_tile<DT, IT, QT, true>(so, acc, a.out, 0, a.m, at, n);
     }
     while (n0 < end) {
       multiply();
-      store_tile<DT, IT, QT, false>(so, acc, a.out, m0, a.m, n0, n);
+      store_tile<DT, IT, QT, false>(so, acc, a.out, 0, a.m, n0, n);
       n0 += 64 * IT;
       if (n0 < end) load(n0);
     }
@@ -389,14 +388,14 @@ __global__ __launch_bounds__(256, QT == 4 ? 2 : 1) void k_cat_stream(StreamArgs 
 #pragma unroll
           for (int j = 0; j < QT; ++j) acc[i][j] = mfma_block(x[i], y[j], acc[i][j], sx[i], sy[j]);
       }
-      store_tile<DT, IT, QT, false>(so, acc, a.out, m0, a.m, n0, n);
+      store_tile<DT, IT, QT, false>(so, acc, a.out, 0, a.m, n0, n);
     }
   }
 }
 
 // a wave's 64 x 64 results, STORE_J 16-query tiles at a time
 template <int DT> constexpr int STORE_J = DT == TT_F32 ? 2 : 4;
-template <int DT, bool WHOLE>
+template <int DT>
 __device__ __forceinline__ void store_wave(uint8_t* so, const f32x4 (&acc)[4][4], void* out, int64_t m0, int64_t m,
                                            int64_t n0, int64_t n) {
   constexpr int J = STORE_J<DT>;
@@ -407,7 +406,7 @@ __device__ __forceinline__ void store_wave(uint8_t* so, const f32x4 (&acc)[4][4]
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < J; ++j) y[i][j] = acc[i][j0 + j];
-    store_tile<DT, 4, J, WHOLE>(so, y, out, m0 + 16 * j0, m, n0, n);
+    store_tile<DT, 4, J, false>(so, y, out, m0 + 16 * j0, m, n0, n);
   }
 }
 
@@ -497,7 +496,7 @@ __global__ __launch_bounds__(256, 3) void k_cat_scores(
     __syncthreads();
   }
 
-  store_wave<DT, false>(lds + w * tile_lds<DT, 4, STORE_J<DT>>(), acc, out, m0 + wm, m, n0 + wn, n);
+  store_wave<DT>(lds + w * tile_lds<DT, 4, STORE_J<DT>>(), acc, out, m0 + wm, m, n0 + wn, n);
 }
 
 // ---------------------------------------------------------------------------

@@ -233,45 +233,35 @@ int64_t tt_cat_scores_workspace_bytes(int64_t m, int64_t n, int32_t d) {
 
 namespace tt {
 template <int DT, int IT, int QT, int NKB>
-static int launch_stream(StreamArgs& a, hipStream_t s) {
-  a.panels = (a.m + 16 * QT - 1) / (16 * QT);
+static void launch_stream(StreamArgs& a, hipStream_t s) {
   const int64_t groups = (a.n + 64 * IT - 1) / (64 * IT);
   // two workgroups a CU, more where each still has four groups to walk over
   const int64_t want = QT == 4 ? 512 : std::max<int64_t>(512, std::min<int64_t>(2048, groups / 4));
-  a.strips = std::max<int64_t>(1, std::min(groups, (want + a.panels - 1) / a.panels));
-  if (a.panels > INT32_MAX / 16 / a.strips) return TT_ERR_UNSUPPORTED;
-  a.per = (a.panels * a.strips + 7) / 8;
+  a.strips = std::min(groups, want);
+  a.per = (a.strips + 7) / 8;
   hipLaunchKernelGGL((k_cat_stream<DT, IT, QT, NKB>), dim3((unsigned)(8 * a.per)), dim3(256), 0, s, a);
-  return TT_OK;
-}
-// queries that the workgroups encode: their codes stay in registers (cat_encodes leaves no other block counts)
-template <int DT, int IT, int QT>
-static int stream_by_blocks(StreamArgs& a, hipStream_t s) {
-  constexpr int MOST = QT == 4 ? 1 : QT == 2 ? 3 : 4;
-  if (a.nkb == 1) return launch_stream<DT, IT, QT, 1>(a, s);
-  if constexpr (MOST >= 2) {
-    if (a.nkb == 2) return launch_stream<DT, IT, QT, 2>(a, s);
-  }
-  if constexpr (MOST >= 3) {
-    if (a.nkb == 3) return launch_stream<DT, IT, QT, 3>(a, s);
-  }
-  if constexpr (MOST >= 4) {
-    if (a.nkb == 4) return launch_stream<DT, IT, QT, 4>(a, s);
-  }
-  return TT_ERR_UNSUPPORTED;
 }
 template <int DT>
 static int launch_scores(StreamArgs& a, hipStream_t s) {
-  if (cat_encodes(a.m, a.nkb)) {
-    if (a.m <= 16) return stream_by_blocks<DT, 1, 1>(a, s);
-    if (a.m <= 32) return stream_by_blocks<DT, 2, 2>(a, s);
-    return stream_by_blocks<DT, 4, 4>(a, s);
+  if (a.m <= 64 && cat_encodes(a.m, a.nkb)) {  // at most 4 blocks a query, 3 of more than 16, 1 of more than 32
+    auto* const f = a.m > 32     ? launch_stream<DT, 4, 4, 1>
+                    : a.m > 16   ? a.nkb == 1   ? launch_stream<DT, 2, 2, 1>
+                                   : a.nkb == 2 ? launch_stream<DT, 2, 2, 2>
+                                                : launch_stream<DT, 2, 2, 3>
+                    : a.nkb == 1 ? launch_stream<DT, 1, 1, 1>
+                    : a.nkb == 2 ? launch_stream<DT, 1, 1, 2>
+                    : a.nkb == 3 ? launch_stream<DT, 1, 1, 3>
+                                 : launch_stream<DT, 1, 1, 4>;
+    f(a, s);
+    return TT_OK;
   }
-  // codes from the workspace, read again for every tile: kept in registers, 24 x 100000 x 384 took 18.4 us for 17.3,
-  // 30 x 100000 x 512 21.6 for 21.7, and 64 x 100000 x 256 went to scratch (35 for 18)
-  if (a.m <= 16) return launch_stream<DT, 1, 1, 0>(a, s);
-  if (a.m <= 32) return launch_stream<DT, 2, 2, 0>(a, s);
-  if (a.m <= 64) return launch_stream<DT, 4, 4, 0>(a, s);
+  if (a.m <= 64) {
+    // codes from the workspace are read again for every tile: kept in registers, 24 x 100000 x 384 took 18.4 us for
+    // 17.3, 30 x 100000 x 512 21.6 for 21.7, and 64 x 100000 x 256 went to scratch (35 for 18)
+    auto* const f = a.m > 32 ? launch_stream<DT, 4, 4, 0> : a.m > 16 ? launch_stream<DT, 2, 2, 0> : launch_stream<DT, 1, 1, 0>;
+    f(a, s);
+    return TT_OK;
+  }
   const int64_t nt = (a.n + CT_N - 1) / CT_N, mt = (a.m + CT_M - 1) / CT_M;
   if (mt > INT32_MAX / 8 / nt) return TT_ERR_UNSUPPORTED;
   const int64_t per = (mt * nt + 7) / 8;
