@@ -325,7 +325,9 @@ static DqPlan dq_plan(int64_t m, int64_t n, int32_t d, int32_t dtype) {
   DqPlan p;
   p.ct = d <= 64 ? 4 : d <= 128 ? 8 : 16;
   p.wm = m <= 16 ? 1 : 4;
-  p.rt = m <= 64 || (dtype == TT_F32 && p.ct == 16) ? 1 : 2;  // what the registers hold
+  // two row tiles a wave where 16 columns of them leave room: with dS in two or three planes they go to scratch (8192 x
+  // 100000 x 256 in fp16 1155 us for 902, 1000 x 20000 x 256 62 for 42; in bf16 541 for 649 with one)
+  p.rt = m <= 64 || (dtype != TT_BF16 && p.ct == 16) ? 1 : 2;
   p.groups = (d + 16 * p.ct - 1) / (16 * p.ct);
   p.mt = (m + 16 * p.rt * p.wm - 1) / (16 * p.rt * p.wm);
   const int64_t step = p.wm == 1 ? 128 : 64, steps = std::max<int64_t>(1, (n + step - 1) / step);
@@ -345,7 +347,8 @@ static void launch_dq_as(const DqArgs& a, hipStream_t s) {
 }
 template <int DT, int DQ, int CT, int RT, int WM>
 static void launch_dq_one(const DqArgs& a, hipStream_t s) {
-  if constexpr (DT != TT_F32) {
+  // 16 columns of two row tiles have no registers for the fifth word (scratch: 8192 x 100001 x 256 832 us for 752)
+  if constexpr (DT != TT_F32 && !(CT == 16 && RT == 2)) {
     if (a.lds % 2 && (uintptr_t)a.ds % 4 == 0 && a.m > 1) return launch_dq_as<DT, DQ, CT, RT, WM, true>(a, s);
   }
   launch_dq_as<DT, DQ, CT, RT, WM, false>(a, s);
@@ -356,7 +359,7 @@ static void launch_dq_rows(const DqArgs& a, const DqPlan& p, hipStream_t s) {
     launch_dq_one<DT, DQ, CT, 1, 1>(a, s);
   else if (p.rt == 1)
     launch_dq_one<DT, DQ, CT, 1, 4>(a, s);
-  else if constexpr (!(DT == TT_F32 && CT == 16))
+  else if constexpr (DT == TT_BF16 || CT < 16)
     launch_dq_one<DT, DQ, CT, 2, 4>(a, s);
 }
 template <int DT, int DQ>
