@@ -235,8 +235,12 @@ namespace tt {
 template <int DT, int IT, int QT, int NKB>
 static void launch_stream(StreamArgs& a, hipStream_t s) {
   const int64_t groups = (a.n + 64 * IT - 1) / (64 * IT);
-  // two workgroups a CU, more where each still has four groups to walk over
-  const int64_t want = QT == 4 ? 512 : std::max<int64_t>(512, std::min<int64_t>(2048, groups / 4));
+  // two workgroups a CU; up to four of the form with the fewest registers, where each has four groups to walk over
+  // (512 / 1024 / 2048 workgroups, us, bf16: 1 x 1000003 x 128 28.8 / 22.6 / 25.9, 1 x 300000 x 128 12.0 / 9.5 / 10.8, 8 x
+  // 1000003 x 60 25.3 / 23.8 / 28.0, 16 x 1000003 x 128 26.8 / 29.0 / 30.9; other forms: 1 x 300000 x 256 15.9 / 17.1 /
+  // 18.7, 16 x 300000 x 512 30.9 / 37.7 / 41.0, 32 x 1000003 x 128 36.1 / 39.4 / 40.0, 37 x 1000003 x 128 42.6 / 42.9 /
+  // 47.9)
+  const int64_t want = QT == 1 && NKB == 1 ? std::max<int64_t>(512, std::min<int64_t>(1024, groups / 4)) : 512;
   a.strips = std::min(groups, want);
   a.per = (a.strips + 7) / 8;
   hipLaunchKernelGGL((k_cat_stream<DT, IT, QT, NKB>), dim3((unsigned)(8 * a.per)), dim3(256), 0, s, a);
