@@ -12,9 +12,9 @@ __device__ __forceinline__ int64_t cat_row(const CatRows& r, int64_t i) { return
 __device__ __forceinline__ bool cat_row_ok(const CatRows& r, int64_t c) { return c >= 0 && c < r.capacity; }
 
 // A row named twice takes its last mention: every mention raises the row's
-// owner to its own place + 1 (k_cat_own), then only the owner writes and puts
-// the word back to zero (k_cat_write); a mention that lost sees either the
-// owner's place or zero, never its own.
+// owner to its own place + 1 (k_cat_own), then only the owner writes
+// (k_cat_write), and every mention puts the word back to zero (k_cat_disown):
+// three launches, 100000 of a million rows of 256 in bf16 28 us.
 __global__ __launch_bounds__(256) void k_cat_own(CatRows r, int64_t m, int32_t* owner) {
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < m; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t c = r.rows[i];
@@ -61,8 +61,9 @@ __global__ __launch_bounds__(256) void k_cat_disown(CatRows r, int64_t m, int32_
 }
 
 // Up to CAT_FEW rows in one launch: every workgroup holds all row numbers in LDS
-// and the 16 lanes of a block look for a later mention of theirs (2 us at 333
-// rows, where three launches took 11)
+// and the 16 lanes of a block look for a later mention of theirs (calls one after
+// the other against three launches, us, 60 values in fp32: 10 rows 3.4 / 6.2, 333
+// 4.2 / 6.7, 1000 6.5 / 7.2)
 constexpr int CAT_FEW = 1024;
 template <int DT>
 __global__ __launch_bounds__(256) void k_cat_write_few(const void* x, int m, int64_t ldx, int d, int nkb, CatRows r,
@@ -421,7 +422,8 @@ constexpr int CT_M = 128, CT_N = 128;
 // takes the x-th eighth of the tiles, in panels of `width` column tiles walked
 // over all row tiles: its L2 holds a panel's catalogue rows (512 KB at most)
 // and meets every query once a panel.  Wide panels also write long pieces of
-// the same rows at a time: 8 -> 32 column tiles 338 -> 273 us at 16384 x 32771 x 128.
+// the same rows at a time.  8 / 16 / 32 / 64 column tiles, us, bf16: 16384 x 32771 x
+// 128 319 / 321 / 272 / 283, 8192 x 100000 x 256 545 / 534 / 585 / 581.
 __device__ __forceinline__ bool cat_tile(int64_t id, int64_t per, int64_t mt, int64_t nt, int width, int64_t& tm,
                                          int64_t& tn) {
   const int64_t t = (id & 7) * per + (id >> 3);
@@ -552,9 +554,9 @@ template <int DT> struct DsFrag {
   u32x4 v[DT == TT_F32 ? 2 : 1];
 };
 // The same as it was loaded.  ODD (16-bit values, rows an odd number of them
-// apart, the first on a 4-byte boundary): loads at 2-byte addresses run at half
-// the rate (428 against 245 us at 16384 x 32771 x 128), so a lane loads the 5
-// words that hold its 8 values and shifts later.  The words reach one value
+// apart, the first on a 4-byte boundary): loads at 2-byte addresses take longer
+// (16384 x 32771 x 128 421 us in bf16, 495 in fp16), so a lane loads the 5 words
+// that hold its 8 values and shifts later (324, 427).  The words reach one value
 // past the 8 and, in odd rows, one before: both are in the array, since the
 // steps that load this way end before the row does.
 template <int DT, bool ODD> struct DsLoad {

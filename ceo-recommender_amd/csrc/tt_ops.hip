@@ -117,8 +117,9 @@ int32_t tt_adamw_step(const tt_adamw_tensor* tensors, int32_t n_tensors, int32_t
   if (state->steps)
     if (const int rc = adamw_advance(tensors, n_tensors, *state, *hp, seed, s)) return rc;
   if (values == 0) return TT_OK;
-  // 8-bit states of many values: 4 rounds a workgroup spare three of four looks for its tensor (96 M values in bf16:
-  // 292 -> 239 us; 32-bit states 517 -> 528 us, small lists want the workgroups)
+  // 8-bit states of many values: 4 rounds a workgroup spare three of four looks for its tensor (one / four rounds, us,
+  // bf16: 1 M values 8.2 / 11.5, 4 M 14.7 / 15.6, 8 M 26.4 / 23.7, 96 M 267 / 215; fp32: 4 M 18.4 / 17.8, 16 M 47.6 /
+  // 46.1; 32-bit states of 96 M 517 / 528)
   const int64_t chunk = ADAMW_STRIDE * (state_bits == 8 && values >= 1 << 22 ? 4 : 1);
   int64_t last_step = 0;
   AdamwCoef last{};
@@ -216,10 +217,11 @@ int32_t tt_cat_read(const uint8_t* codes, const uint8_t* scales, int64_t capacit
 }
 
 // Queries that each streaming workgroup encodes itself, at most 64 blocks in four
-// rounds: no workspace, one launch.  Against a launch for the codes: 20 x 2000 x
-// 128 8.4 / 12.5 us, 64 x 100000 x 128 9.4 / 12.6 us, 37 x 1000003 x 128 39.4 / 42.3
-// us; at 64 blocks of 32-bit results (64 x 100000 x 128) 11.5 / 12.9 us.  More than
-// 64 blocks were not timed.
+// rounds: no workspace, one launch.  Against a launch for the codes, us: 20 x 2000 x
+// 128 4.6 / 6.4, 64 x 100000 x 128 10.8 / 12.3 (32-bit results 12.3 / 13.8), 37 x
+// 1000003 x 128 42.1 / 45.1, 1 x 100000 x 256 7.3 / 9.6, 16 x 50000 x 512 10.7 / 13.4,
+// 21 x 50000 x 384 11.3 / 11.1, 32 x 100000 x 256 12.0 / 15.2 (bf16).  More than 64
+// blocks were not timed.
 static bool cat_encodes(int64_t m, int nkb) { return m * nkb <= 64 && nkb <= 4; }
 
 int64_t tt_cat_scores_workspace_bytes(int64_t m, int64_t n, int32_t d) {
@@ -320,7 +322,10 @@ int32_t tt_cat_scores(const void* q, int32_t dtype, int64_t m, int64_t ldq, int3
 namespace tt {
 // How dq's rows, columns and sum are split.  Parts of the catalogue until about
 // two workgroups a CU have work, none shorter than 2 steps; a part writes m d
-// floats and reads its share of the codes and of dS.
+// floats and reads its share of the codes and of dS.  256 / 512 / 1024 workgroups,
+// in us: 16384 x 32768 x 128 in bf16 326 / 229 / 277, 8192 x 100000 x 256 850 / 536 /
+// 562, 1 x 1000003 x 128 28 / 27 / 31, 64 x 100000 x 256 21 / 25 / 32; 513 x 20011 x
+// 512 in fp32 64 / 64 / 63.
 struct DqPlan {
   int ct, rt, wm, groups;
   int64_t mt, splits, part_steps;
