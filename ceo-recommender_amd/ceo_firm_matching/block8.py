@@ -44,7 +44,9 @@ def encode(x: torch.Tensor):
     b = torch.nn.functional.pad(x.to(torch.float32), (0, -d % BLOCK)).reshape(m, blocks_of(d), BLOCK)
     e = _exponents(b, E4M3[1])
     y = b * torch.exp2(-e.to(torch.float64)).to(torch.float32).unsqueeze(2)
-    y = torch.where(torch.isfinite(b), y, torch.full_like(y, float("nan")))
+    # under the largest scale the code after 240 stands for 2^128, which no float holds: what would round to it stays there
+    most = torch.where(e == 120, 240.0, 448.0).unsqueeze(2)
+    y = torch.where(torch.isfinite(b), torch.minimum(torch.maximum(y, -most), most), torch.full_like(y, float("nan")))
     return y.to(torch.float8_e4m3fn).view(torch.uint8).reshape(m, blocks_of(d) * BLOCK), (e + 127).to(torch.uint8)
 
 

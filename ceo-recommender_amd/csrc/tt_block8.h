@@ -126,14 +126,17 @@ template <int DT>
 __device__ __forceinline__ void st8(void* p, int64_t i, const float (&x)[8]) { stv<DT, 8>(p, i, x); }
 
 // ---- e4m3, rounded to nearest even (the catalogue) -------------------------
-// 8 values under a scale byte -> 8 code bytes; infinities become NaN: e4m3 has none
+// 8 values under a scale byte -> 8 code bytes; infinities become NaN: e4m3 has none.
+// Under the largest scale the code after 240 stands for 2^128, which no float
+// holds: what would round to it stays at 240 (off by 2^-4 of the value at most).
+constexpr uint32_t TOP_BYTE = 247u;
 __device__ __forceinline__ u32x2 encode8_scaled(const float (&x)[8], uint32_t byte) {
-  const float inv = inv_scale(byte);
+  const float inv = inv_scale(byte), most = byte == TOP_BYTE ? 240.f : 448.f;
   float y[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const uint32_t a = __float_as_uint(x[k]) & 0x7FFFFFFFu;
-    y[k] = finite_bits(a) ? x[k] * inv : __uint_as_float(0x7FC00000u);
+    y[k] = finite_bits(a) ? __builtin_amdgcn_fmed3f(x[k] * inv, -most, most) : __uint_as_float(0x7FC00000u);
   }
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);

@@ -525,7 +525,8 @@ int32_t tt_adamw_held(const tt_adamw_state* state, void* m, void* r, tt_stream_t
 /* ---- embedding catalogue in 8 bits (ABI 7) ---------------------------------
  * Rows of d values in e4m3, each block of TT_BLOCK values with a power-of-two
  * scale 2^(byte - 127), the smallest that holds the block's largest finite
- * magnitude (not below 2^-100).  codes [capacity, kp], scales [capacity,
+ * magnitude (not below 2^-100; under the largest, 2^120, codes end at 240,
+ * since 2^128 is no float).  codes [capacity, kp], scales [capacity,
  * kp / TT_BLOCK], kp = d rounded up to TT_BLOCK (padding codes are zero).
  * Infinities and NaN are held as NaN.  Row i of a call is catalogue row
  * rows[i] (device int64), or row0 + i when rows == NULL; rows outside
