@@ -9,10 +9,11 @@
 // chunk counts, one lane a tensor, then walks its chunk.
 //
 // 32-bit states are bound by memory (28 bytes a value in fp32): 96 M values
-// 499 us, 5.4 TB/s.  8-bit states in bf16 (10 bytes a value) by instructions, about
-// 60 a value of which the rounding hash takes 15: 96 M values 236 us; reading the
-// values back (k_adamw_held) 92 us, 6.3 TB/s.  The 21 tensors of the two
-// towers take 3.7 and 4.6 us, launch and latency.
+// 498 us, 5.4 TB/s; in bf16 402 us.  8-bit states in bf16 (10 bytes a value) by
+// instructions, about 60 a value of which the rounding hash takes 15: 96 M values
+// 215-240 us, fp16 224, fp32 302 us (5.1 TB/s); reading the values back
+// (k_adamw_held) 95 us, 6.1 TB/s.  The 21 tensors of the two towers take 3.6 and
+// 4.4 us, launch and latency.
 #include "tt_block8.h"
 
 namespace tt {

@@ -627,9 +627,9 @@ __device__ __forceinline__ void ds_planes(const DsFrag<DT>& f, bf16x8 (&a)[PL]) 
 }
 
 // Bound by dS's bytes up to 128 columns, then by what LDS hands the waves.
-// Measured in bf16: 16384 x 32768 x 128 242 us (4.5 TB/s), x 32771 330 us, 8192 x
-// 100000 x 256 551 us (3.0 TB/s).  16 rows a wave (RT = 1) read LDS twice as often:
-// 826 against 701 us at 8192 x 131072 x 256.
+// Measured in bf16: 16384 x 32768 x 128 238 us (4.5 TB/s), x 32771 324-356 us, 8192
+// x 100000 x 256 540 us (3.0 TB/s; 16 rows a wave read LDS twice as often, 649 us);
+// in fp16 358, 427, 890 us; in fp32 8192 x 32768 x 128 276 us.
 // One workgroup: 16 RT WM rows of dS against a part of the catalogue, 16 CT
 // columns of dq in its waves' accumulators.  A step of DQ_STEP catalogue rows
 // is decoded once into LDS as bf16 [row][column] and read back transposed; the
